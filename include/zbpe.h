@@ -10,7 +10,8 @@
  * Ownership: inputs are borrowed for the duration of a call; outputs go to caller-allocated
  * buffers sized from the arguments; device memory is owned by the context.
  * Threading: one call at a time per context (the reference is single-threaded too).
- * Errors: every entry point returns a zbpe_status; zbpe_last_error() gives the message.
+ * Errors: every entry point returns a zbpe_status; zbpe_last_error() gives the message (of the calling thread's last failed
+ * call without a context, where ctx is NULL).
  */
 #ifndef ZBPE_H
 #define ZBPE_H
@@ -254,6 +255,148 @@ zbpe_status zbpe_halt_log(zbpe_ctx *ctx, uint32_t *rows, size_t cap_rows, size_t
  * second << 16) and count, returns the first pair in slot order whose count == top. */
 zbpe_status zbpe_zig_order_winner(const uint32_t *first_pos, const uint32_t *keys, const uint32_t *counts, size_t n,
                                   uint32_t top, int call_after_last_insert, uint32_t *winner);
+
+/* ---- between a model's logits and its tokens -------------------------------------------------------------------------
+ *
+ * Operators over device buffers of the caller, on the caller's device and stream (a hipStream_t; NULL: the default stream).
+ * They take no context, allocate nothing, wait for nothing (they may be captured into a HIP graph) and may be called from
+ * several threads. On failure zbpe_last_error(NULL) is the calling thread's message. A call whose arguments are refused
+ * launches nothing. Tokens are the ids that zbpe_train makes, so a vocabulary has at most ZBPE_MAX_VOCAB of them.
+ *
+ * Rows: a matrix of logits has `rows` rows of `cols` elements that lie side by side; row r starts
+ * (r / inner) * outer_stride + (r % inner) * inner_stride elements behind `data` (so [batch, time, cols] views with a cut
+ * time axis, and broadcast rows of stride 0, need no copy). Per-row vectors are packed arrays of `rows` elements. */
+#define ZBPE_MAX_VOCAB 65536
+#define ZBPE_MAX_BIASES 1024
+
+typedef enum zbpe_dtype { ZBPE_F32 = 0, ZBPE_F16 = 1, ZBPE_BF16 = 2, ZBPE_I32 = 3, ZBPE_I64 = 4 } zbpe_dtype;
+
+typedef struct zbpe_rows {
+    void *data;
+    int64_t outer_stride, inner_stride; /* in elements */
+    int32_t dtype;                      /* zbpe_dtype */
+} zbpe_rows;
+
+/* Host only. The bytes of every token of a vocabulary, by decode's rules (basic_tokenizer.zig:90-138): a token below 256 is
+ * its byte, any other the first merge that makes it, left half then right half. offsets: vocab_size + 1 u32; token v's bytes
+ * are bytes[offsets[v] .. offsets[v + 1]), none for an id that no merge makes. *n_bytes receives their number; they are
+ * written when cap is at least that. ZBPE_INVALID_TOKEN: a merge uses a token without bytes, or itself.
+ * ZBPE_INVALID_ARGUMENT: vocab_size outside 256 .. ZBPE_MAX_VOCAB, a merge makes a token outside it, or 2^31 bytes or more. */
+zbpe_status zbpe_vocab_bytes(const uint16_t *triples, size_t n_merges, size_t vocab_size, uint32_t *offsets, uint8_t *bytes,
+                             size_t cap, size_t *n_bytes);
+
+/* A grammar over a vocabulary, on the device: an automaton over bytes, and the tokens' bytes (zbpe_vocab_bytes). */
+typedef struct zbpe_grammar {
+    const uint32_t *offsets;  /* [vocab_size + 1] */
+    const uint8_t *bytes;
+    int32_t vocab_size;
+    int32_t end_token;        /* a token that ends an answer: allowed in accepting states only, whatever its bytes; -1: none */
+    const int32_t *next;      /* [n_states][256]: the state after a byte; any value outside 0 .. n_states - 1: refused */
+    const uint8_t *accepting; /* [n_states], or NULL: no state accepts */
+    int32_t n_states;
+} zbpe_grammar;
+
+/* Which tokens the grammar allows: row r of `masks` (words = (vocab_size + 31) / 32 u32) gets bit v % 32 of word v / 32 set
+ * when the automaton reads all of token v's bytes from state states[r] (NULL: state r). Tokens without bytes are not
+ * allowed, nor is any token in a state outside 0 .. n_states - 1. Bits past vocab_size are 0. */
+zbpe_status zbpe_grammar_masks(int device, void *stream, const zbpe_grammar *grammar, const int32_t *states, int64_t rows,
+                               uint32_t *masks);
+
+/* out[r] = the state after tokens[r] from states[r]; -1 when the grammar refuses it, and for a state that is outside the
+ * automaton. A token outside the vocabulary is refused; a negative one (a row that drew nothing) leaves the state as it
+ * is; the end token keeps an accepting state. `out` may be `states`. */
+zbpe_status zbpe_grammar_advance(int device, void *stream, const zbpe_grammar *grammar, const int32_t *states,
+                                 const int32_t *tokens, int64_t rows, int32_t *out);
+
+/* Penalties for repeated tokens, biases and masks on logits. For row r and token v, each step rounded to 32 bits:
+ *   z = logits[r][v]
+ *   v among the row's first lengths[r] history tokens:           z = z > 0 ? z / repetition[r] : z * repetition[r]
+ *   v is there c > 0 times behind the first prompt_lengths[r]:   z = z - frequency[r] * c, then z - presence[r]
+ *   z = z + bias[v];  z = z + (the sum, in order, of the bias_values[r][j] with bias_tokens[r][j] == v)
+ *   the mask's bit is 0:                                          z = -inf, whatever z was
+ * and out[r][v] = z rounded to out's type. History and bias tokens outside the vocabulary are passed over (padding). */
+typedef struct zbpe_adjust {
+    uint32_t struct_size;     /* sizeof(zbpe_adjust) */
+    int32_t cols;             /* 1 .. ZBPE_MAX_VOCAB */
+    int64_t rows, inner;      /* inner >= 1 */
+    zbpe_rows logits;         /* F32, F16 or BF16 */
+    zbpe_rows out;            /* the type of the logits, or F32; may be the logits themselves */
+    zbpe_rows history;        /* I32 or I64; data NULL: none */
+    int64_t history_len;      /* tokens a row has room for */
+    const int32_t *lengths;         /* NULL: history_len; clamped to 0 .. history_len */
+    const int32_t *prompt_lengths;  /* NULL: 0 */
+    const float *repetition, *presence, *frequency; /* NULL: 1, 0, 0 */
+    const float *bias;              /* [cols], or NULL */
+    const int32_t *bias_tokens;     /* [rows][n_biases] */
+    const float *bias_values;       /* [rows][n_biases] */
+    int32_t n_biases;               /* 0 .. ZBPE_MAX_BIASES */
+    int32_t mask_words;             /* u32 from one row of masks to the next, (cols + 31) / 32 at least */
+    const uint32_t *masks;          /* [mask_rows][mask_words], or NULL */
+    int64_t mask_rows;
+    const int32_t *states;          /* the row of masks for each row, outside 0 .. mask_rows - 1: everything masked;
+                                       NULL: row r, or row 0 when mask_rows is 1 */
+} zbpe_adjust;
+
+zbpe_status zbpe_adjust_logits(int device, void *stream, const zbpe_adjust *args);
+
+/* Its gradient: `args` as in the call, args->out the gradient of its output (only read), args->logits the same logits. Writes
+ * grad_logits (the logits' type, rows of its own), grad_bias [cols] and grad_bias_values [rows][n_biases]; each may be NULL.
+ * A masked element passes no gradient. grad_bias needs a workspace of zbpe_adjust_workspace(rows, cols) bytes, which no
+ * other call uses until this one is done; it sums rows in an order that depends on rows and cols alone. */
+size_t zbpe_adjust_workspace(int64_t rows, int32_t cols);
+zbpe_status zbpe_adjust_logits_grad(int device, void *stream, const zbpe_adjust *args, const zbpe_rows *grad_logits,
+                                    float *grad_bias, float *grad_bias_values, void *workspace, size_t workspace_size);
+
+/* One token a row. With w = exp((z - max z) / temperature), and tokens ranked by z, larger first, then by id:
+ *   top_k:  the first top_k ranks stay (0 or less: all)
+ *   top_p:  of these, a token stays when the w before it in rank sum to less than top_p times their whole sum (1 or more: all;
+ *           0 or less: the first rank alone)
+ *   min_p:  and when its w is at least min_p (0 or less: all; above 1 is 1)
+ * the token is the first, by id, at which the sum of the kept w exceeds uniforms[r] times the whole; logprobs[r] is the
+ * logarithm of its share. A temperature of 0 or less (or NaN) takes the first rank, with log-probability 0. NaN logits are
+ * never drawn; nor are -inf ones, and a row with nothing else gets token -1 and log-probability -inf. Where the largest is
+ * +inf, only such tokens have weight. Weights are held in steps of 2^-47 of the largest: sums are exact, whatever their
+ * order, and a weight below half a step is none. uniforms in [0, 1); what lies outside is taken as the nearest inside. */
+typedef struct zbpe_draw {
+    uint32_t struct_size;     /* sizeof(zbpe_draw) */
+    int32_t cols;
+    int64_t rows, inner;
+    zbpe_rows logits;         /* F32, F16 or BF16 */
+    const float *uniforms;
+    const float *temperature; /* NULL: 1 */
+    const int32_t *top_k;     /* NULL: 0 */
+    const float *top_p;       /* NULL: 1 */
+    const float *min_p;       /* NULL: 0 */
+    int32_t *tokens;
+    float *logprobs;          /* or NULL */
+} zbpe_draw;
+
+zbpe_status zbpe_draw_tokens(int device, void *stream, const zbpe_draw *args);
+
+/* logprobs[r] = z[t] - log sum_v exp(z[v]) with z = logits[r] / temperature[r], t = tokens[r] (I32 or I64, packed). A negative
+ * token is not scored: 0, and no gradient. A token past the last column gives NaN. A row without anything above -inf gives
+ * -inf and no gradient. stats ([rows][2] f32: the row's maximum, and the sum of exp(z - its maximum)) is what the gradient
+ * needs; it may be NULL when none follows. temperature: NULL: 1; positive.
+ * zbpe_token_logprobs_grad writes grad_logits (the logits' type) = grad[r] / temperature[r] * ([v == t] - softmax(z)[v]). */
+typedef struct zbpe_logprobs {
+    uint32_t struct_size;     /* sizeof(zbpe_logprobs) */
+    int32_t cols;
+    int64_t rows, inner;
+    zbpe_rows logits;         /* F32, F16 or BF16 */
+    const void *tokens;
+    int32_t tokens_dtype;     /* ZBPE_I32 or ZBPE_I64 */
+    const float *temperature;
+    float *logprobs;          /* written (read by nothing in the gradient's call) */
+    float *stats;             /* written; read in the gradient's call */
+} zbpe_logprobs;
+
+zbpe_status zbpe_token_logprobs(int device, void *stream, const zbpe_logprobs *args);
+zbpe_status zbpe_token_logprobs_grad(int device, void *stream, const zbpe_logprobs *args, const float *grad,
+                                     const zbpe_rows *grad_logits);
+
+/* sizeof(zbpe_adjust), sizeof(zbpe_draw), sizeof(zbpe_logprobs), sizeof(zbpe_grammar) as the library was built, for which = 0 .. 3
+ * (0 for any other): a consumer compares them with its own header's. */
+size_t zbpe_struct_size(int which);
 
 /* Library version string. */
 const char *zbpe_version(void);

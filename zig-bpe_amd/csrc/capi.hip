@@ -5,6 +5,7 @@
 #include <new>
 
 #include "engine.hpp"
+#include "logits.hpp"
 #include "zig_order.hpp"
 #include <vector>
 #include <string>
@@ -79,7 +80,11 @@ zbpe_status zbpe_create_dist_host(int device, int rank, int world, zbpe_collecti
 
 void zbpe_destroy(zbpe_ctx *ctx) { delete ctx; }
 
-const char *zbpe_last_error(const zbpe_ctx *ctx) { return ctx ? ctx->eng.err.c_str() : "null context"; }
+const char *zbpe_last_error(const zbpe_ctx *ctx) {
+    if (ctx) return ctx->eng.err.c_str();
+    const char *m = zbpe::thread_message();
+    return m ? m : "null context";
+}
 
 zbpe_status zbpe_upload(zbpe_ctx *ctx, const uint8_t *text, size_t n) {
     if (!ctx || (!text && n)) return ZBPE_INVALID_ARGUMENT;

@@ -1,0 +1,1035 @@
+// The operators between a model's logits and its tokens (include/zbpe.h): grammar masks over the vocabulary, penalties /
+// biases / masks on logits and their gradient, the draw of a token, log-probabilities and their gradient.
+#include <hip/hip_runtime.h>
+#include <stdarg.h>
+#include <stdint.h>
+#include <stdio.h>
+
+#include <exception>
+#include <new>
+
+#include "../../include/zbpe.h"
+#include "logits.hpp"
+#include "vocab.hpp"
+
+namespace zbpe {
+
+static thread_local char g_message[512] = "";
+const char *thread_message() { return g_message[0] ? g_message : nullptr; }
+
+__attribute__((format(printf, 2, 3))) static zbpe_status refuse(zbpe_status s, const char *fmt, ...) {
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(g_message, sizeof g_message, fmt, ap);
+    va_end(ap);
+    return s;
+}
+
+// ---- rows ---------------------------------------------------------------------------------------------------------------
+
+// One matrix of a launch: where row r starts.
+struct Rows {
+    char *data;
+    int64_t outer, inner;  // strides, in elements
+};
+template <class T>
+__device__ __forceinline__ T *row_of(const Rows &m, int64_t r, int64_t per) {
+    // (the common case of one stride: no division)
+    const int64_t at = m.outer == per * m.inner ? r * m.inner : (r / per) * m.outer + (r % per) * m.inner;
+    return (T *)m.data + at;
+}
+
+using f16 = _Float16;
+using bf16 = __bf16;
+
+// 16 bytes of elements. Rows may start at any element (an odd number of columns): the copies below are 16-byte loads and
+// stores at the element's alignment, which global memory allows.
+template <class T>
+struct Pack {
+    static constexpr int N = 16 / sizeof(T);
+    T v[N];
+};
+template <class T>
+__device__ __forceinline__ Pack<T> load_pack(const T *p) {
+    Pack<T> x;
+    __builtin_memcpy(&x, p, sizeof x);
+    return x;
+}
+// N consecutive elements as floats; those past `cols` become `fill`.
+template <class T, int N>
+__device__ __forceinline__ void load_floats(const T *row, int col, int cols, float fill, float *z) {
+    static_assert(N % Pack<T>::N == 0, "whole packs");
+    if (col + N <= cols) {
+#pragma unroll
+        for (int k = 0; k < N; k += Pack<T>::N) {
+            const Pack<T> x = load_pack(row + col + k);
+#pragma unroll
+            for (int e = 0; e < Pack<T>::N; e++) z[k + e] = (float)x.v[e];
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; e++) z[e] = col + e < cols ? (float)row[col + e] : fill;
+    }
+}
+template <class T, int N>
+__device__ __forceinline__ void store_floats(T *row, int col, int cols, const float *z) {
+    if (col + N <= cols) {
+        T x[N];
+#pragma unroll
+        for (int e = 0; e < N; e++) x[e] = (T)z[e];
+        __builtin_memcpy(row + col, x, sizeof x);
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; e++)
+            if (col + e < cols) row[col + e] = (T)z[e];
+    }
+}
+
+constexpr float INF = __builtin_huge_valf();
+
+// ---- wave and workgroup sums --------------------------------------------------------------------------------------------
+
+__device__ __forceinline__ float wave_max(float x) {
+    for (int d = 32; d; d >>= 1) x = fmaxf(x, __shfl_xor(x, d));
+    return x;
+}
+__device__ __forceinline__ float wave_sum(float x) {
+    for (int d = 32; d; d >>= 1) x += __shfl_xor(x, d);
+    return x;
+}
+__device__ __forceinline__ uint64_t wave_sum(uint64_t x) {
+    for (int d = 32; d; d >>= 1) x += __shfl_xor((unsigned long long)x, d);
+    return x;
+}
+__device__ __forceinline__ int wave_min(int x) {
+    for (int d = 32; d; d >>= 1) x = min(x, __shfl_xor(x, d));
+    return x;
+}
+__device__ __forceinline__ uint64_t wave_scan(uint64_t x) {  // inclusive
+    const int lane = threadIdx.x & 63;
+    for (int d = 1; d < 64; d <<= 1) {
+        const uint64_t y = __shfl_up((unsigned long long)x, d);
+        if (lane >= d) x += y;
+    }
+    return x;
+}
+
+// ---- grammar masks ------------------------------------------------------------------------------------------------------
+
+struct Automaton {
+    const uint32_t *offsets;
+    const uint8_t *bytes;
+    const int32_t *next;
+    const uint8_t *accepting;
+    int vocab, end, n;
+};
+
+__device__ __forceinline__ bool inside(const Automaton &g, int s) { return (uint32_t)s < (uint32_t)g.n; }
+
+// The state after bytes [at, to) from s; -1 once it is outside the automaton.
+__device__ __forceinline__ int walk(const Automaton &g, int s, uint32_t at, uint32_t to) {
+    while (at < to && inside(g, s)) s = g.next[(int64_t)s * 256 + g.bytes[at++]];
+    return inside(g, s) ? s : -1;
+}
+
+__global__ __launch_bounds__(256) void grammar_masks_kernel(Automaton g, const int32_t *states, int64_t rows, uint32_t *masks, int slices) {
+    const int words = (g.vocab + 31) / 32, lane = threadIdx.x & 63;
+    for (int64_t w = blockIdx.x; w < rows * slices; w += gridDim.x) {
+        const int64_t r = w / slices;
+        const int v = (int)(w % slices) * 256 + (int)threadIdx.x;
+        const int s = states ? states[r] : (int)r;
+        bool on = false;
+        if (v < g.vocab && inside(g, s)) {
+            if (v == g.end) on = g.accepting && g.accepting[s];
+            else {
+                const uint32_t a = g.offsets[v], b = g.offsets[v + 1];
+                on = a < b && walk(g, s, a, b) >= 0;
+            }
+        }
+        const uint64_t bits = __ballot(on);
+        const int word = (v - lane) / 32 + (lane >> 5);
+        if ((lane & 31) == 0 && word < words) masks[r * words + word] = (uint32_t)(bits >> (lane & 32));
+    }
+}
+
+__global__ __launch_bounds__(256) void grammar_advance_kernel(Automaton g, const int32_t *states, const int32_t *tokens, int64_t rows, int32_t *out) {
+    for (int64_t r = blockIdx.x * 256ll + threadIdx.x; r < rows; r += gridDim.x * 256ll) {
+        const int s = states[r], v = tokens[r];
+        int to = -1;
+        if (inside(g, s)) {
+            if (v < 0) to = s;
+            else if (v >= g.vocab) to = -1;
+            else if (v == g.end) to = g.accepting && g.accepting[s] ? s : -1;
+            else if (g.offsets[v] < g.offsets[v + 1]) to = walk(g, s, g.offsets[v], g.offsets[v + 1]);
+        }
+        out[r] = to;
+    }
+}
+
+// ---- penalties, biases and masks ----------------------------------------------------------------------------------------
+
+constexpr int ADJUST_THREADS = 256, ADJUST_EACH = 16, ADJUST_SLICE = ADJUST_THREADS * ADJUST_EACH;
+
+struct Adjust {
+    Rows logits, out, history;
+    int64_t rows, inner, mask_rows;
+    int cols, slices, words, n_biases, wide_ids;
+    int64_t history_len;
+    const int32_t *lengths, *prompt_lengths, *bias_tokens, *states;
+    const float *repetition, *presence, *frequency, *bias, *bias_values;
+    const uint32_t *masks;
+};
+
+// The row of masks of logits row r; null: everything is masked.
+__device__ __forceinline__ const uint32_t *mask_row(const Adjust &a, int64_t r) {
+    const int64_t m = a.states ? a.states[r] : a.mask_rows == 1 ? 0 : r;
+    return m >= 0 && m < a.mask_rows ? a.masks + m * a.words : nullptr;
+}
+
+template <class F>
+__device__ __forceinline__ void each_history(const Adjust &a, int64_t r, F f) {
+    int64_t n = a.lengths ? a.lengths[r] : a.history_len;
+    n = n < 0 ? 0 : n > a.history_len ? a.history_len : n;
+    if (a.wide_ids) {
+        const int64_t *ids = row_of<int64_t>(a.history, r, a.inner);
+        for (int64_t i = threadIdx.x; i < n; i += ADJUST_THREADS) f(i, ids[i]);
+    } else {
+        const int32_t *ids = row_of<int32_t>(a.history, r, a.inner);
+        for (int64_t i = threadIdx.x; i < n; i += ADJUST_THREADS) f(i, (int64_t)ids[i]);
+    }
+}
+
+constexpr uint32_t SEEN = 1u << 31;  // of a cell: the token is in the history; below it, how often behind the prompt
+
+template <class Ti, class To>
+__global__ __launch_bounds__(ADJUST_THREADS) void adjust_kernel(Adjust a) {
+#pragma clang fp contract(off)
+    __shared__ uint32_t cell[ADJUST_SLICE];
+    __shared__ float extra[ADJUST_SLICE];
+    const int t = threadIdx.x;
+    for (int64_t w = blockIdx.x; w < a.rows * a.slices; w += gridDim.x) {
+        const int64_t r = w / a.slices;
+        const int base = (int)(w % a.slices) * ADJUST_SLICE;
+        const bool past = a.history.data != nullptr, biased = a.n_biases > 0;
+        if (past || biased) {
+            __syncthreads();
+            for (int i = t; i < ADJUST_SLICE; i += ADJUST_THREADS) {
+                cell[i] = 0;
+                extra[i] = 0.0f;
+            }
+            __syncthreads();
+            if (past) {
+                const int64_t prompt = a.prompt_lengths ? a.prompt_lengths[r] : 0;
+                each_history(a, r, [&](int64_t i, int64_t id) {
+                    const int64_t k = id - base;
+                    if (k < 0 || k >= ADJUST_SLICE) return;
+                    atomicOr(&cell[k], SEEN);
+                    if (i >= prompt) atomicAdd(&cell[k], 1u);
+                });
+            }
+            // the first entry of a token sums all of its row's entries, in their order
+            for (int j = t; j < a.n_biases; j += ADJUST_THREADS) {
+                const int32_t *ids = a.bias_tokens + r * a.n_biases;
+                const float *value = a.bias_values + r * a.n_biases;
+                const int64_t k = (int64_t)ids[j] - base;
+                if (k < 0 || k >= ADJUST_SLICE) continue;
+                bool first = true;
+                for (int i = 0; i < j && first; i++) first = ids[i] != ids[j];
+                if (!first) continue;
+                float sum = value[j];
+                for (int i = j + 1; i < a.n_biases; i++)
+                    if (ids[i] == ids[j]) sum += value[i];
+                extra[k] = sum;
+            }
+            __syncthreads();
+        }
+        const float theta = a.repetition ? a.repetition[r] : 1.0f;
+        const float presence = a.presence ? a.presence[r] : 0.0f, frequency = a.frequency ? a.frequency[r] : 0.0f;
+        const uint32_t *mask = a.masks ? mask_row(a, r) : nullptr;
+        const Ti *in = row_of<Ti>(a.logits, r, a.inner);
+        To *out = row_of<To>(a.out, r, a.inner);
+        constexpr int N = Pack<Ti>::N;
+#pragma unroll
+        for (int c = 0; c < ADJUST_EACH / N; c++) {
+            const int k = (c * ADJUST_THREADS + t) * N, col = base + k;
+            if (col >= a.cols) continue;
+            float z[N];
+            load_floats<Ti, N>(in, col, a.cols, 0.0f, z);
+            uint32_t allowed = ~0u;
+            if (a.masks) allowed = mask ? mask[col >> 5] >> (col & 31) : 0u;  // (col is a multiple of N: one word holds them)
+#pragma unroll
+            for (int e = 0; e < N; e++) {
+                float y = z[e];
+                if (past) {
+                    const uint32_t seen = cell[k + e];
+                    if (seen) {
+                        y = y > 0.0f ? y / theta : y * theta;
+                        const uint32_t count = seen & ~SEEN;
+                        if (count) {
+                            y = y - frequency * (float)count;
+                            y = y - presence;
+                        }
+                    }
+                }
+                if (a.bias) y = y + (col + e < a.cols ? a.bias[col + e] : 0.0f);
+                if (biased) y = y + extra[k + e];
+                z[e] = (allowed >> e) & 1 ? y : -INF;
+            }
+            store_floats<To, N>(out, col, a.cols, z);
+        }
+    }
+}
+
+// dz = dy * slope, masked; the sum over rows of the masked dy for the shared bias. One workgroup takes a slice of columns
+// and a run of rows, keeps its columns' sums in registers over the run, and leaves them in the workspace; a second
+// kernel adds the runs up in their order.
+struct AdjustGrad {
+    Adjust a;  // a.out: the gradient of the output
+    Rows grad_logits;
+    float *grad_bias_values, *sums;
+    int run, runs;
+};
+
+template <class Ti, class To>
+__global__ __launch_bounds__(ADJUST_THREADS) void adjust_grad_kernel(AdjustGrad g) {
+    const Adjust &a = g.a;
+    __shared__ uint32_t seen[ADJUST_SLICE / 32];
+    const int t = threadIdx.x;
+    constexpr int N = Pack<Ti>::N, C = ADJUST_EACH / N;
+    for (int64_t w = blockIdx.x; w < (int64_t)g.runs * a.slices; w += gridDim.x) {
+        const int64_t first = w / a.slices * g.run, last = first + g.run < a.rows ? first + g.run : a.rows;
+        const int slice = (int)(w % a.slices), base = slice * ADJUST_SLICE;
+        const bool past = a.history.data != nullptr;
+        float sum[ADJUST_EACH] = {};
+        for (int64_t r = first; r < last; r++) {
+            if (past) {
+                __syncthreads();
+                for (int i = t; i < ADJUST_SLICE / 32; i += ADJUST_THREADS) seen[i] = 0;
+                __syncthreads();
+                each_history(a, r, [&](int64_t, int64_t id) {
+                    const int64_t k = id - base;
+                    if (k >= 0 && k < ADJUST_SLICE) atomicOr(&seen[k >> 5], 1u << (k & 31));
+                });
+                __syncthreads();
+            }
+            const float theta = a.repetition ? a.repetition[r] : 1.0f;
+            const uint32_t *mask = a.masks ? mask_row(a, r) : nullptr;
+            const Ti *in = row_of<Ti>(a.logits, r, a.inner);
+            const To *up = row_of<To>(a.out, r, a.inner);
+            Ti *down = g.grad_logits.data ? row_of<Ti>(g.grad_logits, r, a.inner) : nullptr;
+#pragma unroll
+            for (int c = 0; c < C; c++) {
+                const int k = (c * ADJUST_THREADS + t) * N, col = base + k;
+                if (col >= a.cols) continue;
+                float d[N];
+                load_floats<To, N>(up, col, a.cols, 0.0f, d);
+                uint32_t allowed = ~0u;
+                if (a.masks) allowed = mask ? mask[col >> 5] >> (col & 31) : 0u;
+                const uint32_t old = past ? seen[k >> 5] >> (k & 31) : 0u;
+#pragma unroll
+                for (int e = 0; e < N; e++) {
+                    d[e] = (allowed >> e) & 1 ? d[e] : 0.0f;
+                    sum[c * N + e] += d[e];
+                    if ((old >> e) & 1 && col + e < a.cols) d[e] = (float)in[col + e] > 0.0f ? d[e] / theta : d[e] * theta;
+                }
+                if (down) store_floats<Ti, N>(down, col, a.cols, d);
+            }
+            if (g.grad_bias_values)
+                for (int j = t; j < a.n_biases; j += ADJUST_THREADS) {
+                    const int32_t id = a.bias_tokens[r * a.n_biases + j];
+                    float d = 0.0f;
+                    if (id < 0 || id >= a.cols) {
+                        if (slice) continue;  // (no slice holds it: the first one writes its 0)
+                    } else {
+                        if (id / ADJUST_SLICE != slice) continue;
+                        if (!a.masks || (mask && (mask[id >> 5] >> (id & 31)) & 1)) d = (float)up[id];
+                    }
+                    g.grad_bias_values[r * a.n_biases + j] = d;
+                }
+        }
+        if (g.sums)
+#pragma unroll
+            for (int c = 0; c < C; c++)
+#pragma unroll
+                for (int e = 0; e < N; e++) {
+                    const int col = base + (c * ADJUST_THREADS + t) * N + e;
+                    if (col < a.cols) g.sums[w / a.slices * a.cols + col] = sum[c * N + e];
+                }
+    }
+}
+
+__global__ __launch_bounds__(256) void adjust_bias_kernel(const float *sums, int runs, int cols, float *grad_bias) {
+    const int col = blockIdx.x * 64 + (threadIdx.x & 63), part = threadIdx.x >> 6;
+    __shared__ float other[3][64];
+    float s = 0.0f;
+    if (col < cols)
+        for (int i = part; i < runs; i += 4) s += sums[(int64_t)i * cols + col];
+    if (part) other[part - 1][threadIdx.x & 63] = s;
+    __syncthreads();
+    if (!part && col < cols) grad_bias[col] = ((s + other[0][threadIdx.x]) + other[1][threadIdx.x]) + other[2][threadIdx.x];
+}
+
+// ---- the draw -----------------------------------------------------------------------------------------------------------
+
+struct Draw {
+    Rows logits;
+    int64_t rows, inner;
+    int cols;
+    const float *uniforms, *temperature, *top_p, *min_p;
+    const int32_t *top_k;
+    int32_t *tokens;
+    float *logprobs;
+};
+
+// A float's place in the order of values, as an unsigned number.
+__device__ __forceinline__ uint32_t key_of(float z) {
+    const uint32_t b = __float_as_uint(z);
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
+
+// One workgroup keeps a row in registers (NE values a thread) and goes over it as often as the filters need.
+template <class T, int NT, int NE>
+struct Drawer {
+    static constexpr int N = Pack<T>::N, C = NE / N, W = NT / 64, SEGMENTS = C * W;
+    struct Shared {
+        uint64_t start[SEGMENTS];  // the sum of the weights in front of each segment (chunk c of wave w: c * W + w, in id order)
+        uint64_t mass[256];
+        uint64_t total, base;
+        float maxima[W];
+        int col, bin;
+    };
+    float z[NE];
+    Shared &sh;
+    int cols;
+    float top;         // the row's maximum
+    double inverse;    // 1 / temperature
+    uint32_t cut_key;  // kept: a larger key, or this one up to cut_col
+    int cut_col;
+
+    __device__ __forceinline__ static int col_of(int c, int e) { return (c * NT + (int)threadIdx.x) * N + e; }
+    __device__ __forceinline__ bool kept(float v, int col) const {
+        const uint32_t k = key_of(v);
+        return v > -INF && (k > cut_key || (k == cut_key && col <= cut_col));
+    }
+    __device__ __forceinline__ double weight(float v) const {
+        return v == top ? 1.0 : top == INF ? 0.0 : exp(((double)v - (double)top) * inverse);
+    }
+    // 2^47 w rounded: w + 32 has steps of 2^-47, and its mantissa is the multiple
+    __device__ __forceinline__ static uint64_t steps(double w) {
+        return (uint64_t)__double_as_longlong(w + 32.0) & ((1ull << 52) - 1);
+    }
+
+    __device__ __forceinline__ void load(const T *row) {
+#pragma unroll
+        for (int c = 0; c < C; c++) load_floats<T, N>(row, col_of(c, 0), cols, -INF, z + c * N);
+        float m = -INF;
+#pragma unroll
+        for (int i = 0; i < NE; i++) {
+            z[i] = z[i] == z[i] ? z[i] + 0.0f : -INF;  // (+ 0: one key for both zeros)
+            m = fmaxf(m, z[i]);
+        }
+        m = wave_max(m);
+        if ((threadIdx.x & 63) == 0) sh.maxima[threadIdx.x >> 6] = m;
+        __syncthreads();
+        top = -INF;
+#pragma unroll
+        for (int w = 0; w < W; w++) top = fmaxf(top, sh.maxima[w]);
+        cut_key = 0;
+        cut_col = 1 << 30;
+    }
+
+    // Sums f(value, column) over the row in id order; leaves the sums in front of each segment in `start`.
+    template <class F>
+    __device__ __forceinline__ uint64_t total(F f) {
+        const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+        __syncthreads();
+#pragma unroll
+        for (int c = 0; c < C; c++) {
+            uint64_t s = 0;
+#pragma unroll
+            for (int e = 0; e < N; e++) s += f(z[c * N + e], col_of(c, e));
+            s = wave_sum(s);
+            if (lane == 0) sh.start[c * W + wave] = s;
+        }
+        __syncthreads();
+        if (wave == 0) {
+            constexpr int EACH = (SEGMENTS + 63) / 64;
+            uint64_t own[EACH], s = 0;
+#pragma unroll
+            for (int i = 0; i < EACH; i++) {
+                own[i] = lane * EACH + i < SEGMENTS ? sh.start[lane * EACH + i] : 0;
+                s += own[i];
+            }
+            uint64_t at = wave_scan(s) - s;
+#pragma unroll
+            for (int i = 0; i < EACH; i++) {
+                if (lane * EACH + i < SEGMENTS) sh.start[lane * EACH + i] = at;
+                at += own[i];
+            }
+            if (lane == 63) sh.total = at;
+        }
+        __syncthreads();
+        return sh.total;
+    }
+
+    // After total(f): the first column at which the sum of f, that column included, exceeds t (t < the total).
+    template <class F>
+    __device__ __forceinline__ int locate(uint64_t t, F f) {
+        const int wave = threadIdx.x >> 6;
+#pragma unroll
+        for (int c = 0; c < C; c++) {
+            const int seg = c * W + wave;
+            const uint64_t from = sh.start[seg], to = seg + 1 < SEGMENTS ? sh.start[seg + 1] : sh.total;
+            if (from <= t && t < to) {  // (one segment of one wave)
+                uint64_t s = 0;
+#pragma unroll
+                for (int e = 0; e < N; e++) s += f(z[c * N + e], col_of(c, e));
+                uint64_t at = from + wave_scan(s) - s;
+                if (at <= t && t < at + s) {
+                    bool open = true;
+#pragma unroll
+                    for (int e = 0; e < N; e++) {
+                        at += f(z[c * N + e], col_of(c, e));
+                        if (open && at > t) {
+                            open = false;
+                            sh.col = col_of(c, e);
+                        }
+                    }
+                }
+            }
+        }
+        __syncthreads();
+        return sh.col;
+    }
+
+    // Moves the cut to the last of the first ranks whose f sum to `target` or more (0 < target <= the sum over what is kept).
+    // f depends on the value alone. Eight bits of the key at a time.
+    template <class F>
+    __device__ __forceinline__ void cut_at(uint64_t target, F f) {
+        uint32_t found = 0;
+        uint64_t base = 0;
+        for (int shift = 24; shift >= 0; shift -= 8) {
+            __syncthreads();
+            for (int i = threadIdx.x; i < 256; i += NT) sh.mass[i] = 0;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < NE; i++) {
+                const uint32_t k = key_of(z[i]);
+                if (kept(z[i], col_of(i / N, i % N)) && (shift == 24 || k >> (shift + 8) == found))
+                    atomicAdd((unsigned long long *)&sh.mass[(k >> shift) & 255], (unsigned long long)f(z[i]));
+            }
+            __syncthreads();
+            if (threadIdx.x < 64) {
+                uint64_t own[4], s = 0;
+#pragma unroll
+                for (int i = 0; i < 4; i++) s += own[i] = sh.mass[255 - (4 * threadIdx.x + i)];
+                uint64_t at = base + wave_scan(s) - s;
+                if (at < target && target <= at + s) {
+                    bool open = true;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        if (open && target <= at + own[i]) {
+                            open = false;
+                            sh.bin = 255 - (4 * (int)threadIdx.x + i);
+                            sh.base = at;
+                        }
+                        at += own[i];
+                    }
+                }
+            }
+            __syncthreads();
+            found = found << 8 | (uint32_t)sh.bin;
+            base = sh.base;
+        }
+        // of the values equal to the cut's, the first by id
+        const uint64_t each = f(of_key(found)), ties = (target - base + each - 1) / each;
+        auto tie = [&](float v, int col) -> uint64_t { return key_of(v) == found && kept(v, col) ? 1 : 0; };
+        total(tie);
+        const int col = locate(ties - 1, tie);
+        cut_key = found;
+        cut_col = col;
+    }
+};
+
+template <class T, int NT, int NE>
+__global__ __launch_bounds__(NT) void draw_kernel(Draw a) {
+    using D = Drawer<T, NT, NE>;
+    __shared__ typename D::Shared sh;
+    for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+        __syncthreads();
+        D d{{}, sh, a.cols, 0.0f, 0.0, 0u, 0};
+        d.load(row_of<T>(a.logits, r, a.inner));
+        const float temperature = a.temperature ? a.temperature[r] : 1.0f;
+        if (!(d.top > -INF)) {
+            if (threadIdx.x == 0) {
+                a.tokens[r] = -1;
+                if (a.logprobs) a.logprobs[r] = -INF;
+            }
+            continue;
+        }
+        if (!(temperature > 0.0f)) {
+            auto first = [&](float v, int) -> uint64_t { return v == d.top ? 1 : 0; };
+            d.total(first);
+            const int col = d.locate(0, first);
+            if (threadIdx.x == 0) {
+                a.tokens[r] = col;
+                if (a.logprobs) a.logprobs[r] = 0.0f;
+            }
+            continue;
+        }
+        d.inverse = 1.0 / (double)temperature;
+        auto one = [&](float v) -> uint64_t { return 1; };
+        auto mass = [&](float v) -> uint64_t { return d.steps(d.weight(v)); };
+        const int k = a.top_k ? a.top_k[r] : 0;
+        if (k > 0 && k < a.cols) {
+            const uint64_t n = d.total([&](float v, int col) -> uint64_t { return d.kept(v, col) ? 1 : 0; });
+            if ((uint64_t)k < n) d.cut_at((uint64_t)k, one);
+        }
+        const float p = a.top_p ? a.top_p[r] : 1.0f;
+        if (p < 1.0f) {
+            const uint64_t whole = d.total([&](float v, int col) -> uint64_t { return d.kept(v, col) ? mass(v) : 0; });
+            uint64_t target = p > 0.0f ? (uint64_t)ceil((double)p * (double)whole) : 1;
+            target = target < 1 ? 1 : target > whole ? whole : target;
+            d.cut_at(target, mass);
+        }
+        const float least_f = a.min_p ? a.min_p[r] : 0.0f;
+        const double least = least_f > 0.0f ? least_f < 1.0f ? (double)least_f : 1.0 : 0.0;
+        auto share = [&](float v, int col) -> uint64_t {
+            if (!d.kept(v, col)) return 0;
+            const double w = d.weight(v);
+            return w >= least ? d.steps(w) : 0;
+        };
+        const uint64_t whole = d.total(share);
+        // u * whole without rounding: u < 1 is a multiple of 2^-64 here (24 bits), and the product's high half its floor
+        const float u = a.uniforms[r];
+        const uint64_t scaled = u >= 1.0f ? ~0ull : u > 0.0f ? (uint64_t)((double)u * 18446744073709551616.0) : 0ull;
+        const int col = d.locate(__umul64hi(whole, scaled), share);
+        if (threadIdx.x == 0) {
+            a.tokens[r] = col;
+            if (a.logprobs) {
+                const float v = (float)row_of<T>(a.logits, r, a.inner)[col];
+                const double x = v == d.top ? 0.0 : ((double)v - (double)d.top) * d.inverse;
+                a.logprobs[r] = (float)(x - log((double)whole * 0x1p-47));
+            }
+        }
+    }
+}
+
+// ---- log-probabilities --------------------------------------------------------------------------------------------------
+
+struct Logprobs {
+    Rows logits, grad_logits;
+    int64_t rows, inner;
+    int cols, wide_ids;
+    const void *tokens;
+    const float *temperature, *grad;
+    float *logprobs, *stats;
+};
+
+constexpr float LOG2E = 1.44269504088896340736f;
+
+__device__ __forceinline__ int64_t token_of(const Logprobs &a, int64_t r) {
+    return a.wide_ids ? ((const int64_t *)a.tokens)[r] : (int64_t)((const int32_t *)a.tokens)[r];
+}
+
+// One pass with a running maximum and sum. TPR threads go over one row.
+template <class T, int TPR>
+__global__ __launch_bounds__(256) void logprobs_kernel(Logprobs a) {
+    constexpr int N = Pack<T>::N, PER = 256 / TPR;
+    __shared__ float maxima[4], sums[4];
+    const int t = threadIdx.x % TPR;
+    for (int64_t r0 = blockIdx.x * (int64_t)PER; r0 < a.rows; r0 += gridDim.x * (int64_t)PER) {
+        const int64_t r = r0 + threadIdx.x / TPR;
+        const bool on = r < a.rows;
+        const float temperature = on && a.temperature ? a.temperature[r] : 1.0f;
+        const float inverse = 1.0f / temperature, scale = inverse * LOG2E;
+        const T *row = on ? row_of<T>(a.logits, r, a.inner) : nullptr;
+        float m = -INF, s = 0.0f;
+        if (on)
+            for (int col = t * N; col < a.cols; col += TPR * N) {
+                float z[N];
+                load_floats<T, N>(row, col, a.cols, -INF, z);
+                float more = m;
+#pragma unroll
+                for (int e = 0; e < N; e++) more = fmaxf(more, z[e]);
+                const float from = more == -INF ? 0.0f : more;  // (nothing yet above -inf: the exponentials are 0, not NaN)
+                s *= __builtin_amdgcn_exp2f((m - from) * scale);
+#pragma unroll
+                for (int e = 0; e < N; e++) s += __builtin_amdgcn_exp2f((z[e] - from) * scale);
+                m = more;
+            }
+        float top = wave_max(m);
+        s = wave_sum(s * __builtin_amdgcn_exp2f((m - (top == -INF ? 0.0f : top)) * scale));
+        if (TPR > 64) {
+            __syncthreads();
+            if ((threadIdx.x & 63) == 0) {
+                maxima[threadIdx.x >> 6] = top;
+                sums[threadIdx.x >> 6] = s;
+            }
+            __syncthreads();
+            top = fmaxf(fmaxf(maxima[0], maxima[1]), fmaxf(maxima[2], maxima[3]));
+            const float from = top == -INF ? 0.0f : top;
+            s = 0.0f;
+#pragma unroll
+            for (int w = 0; w < 4; w++) s += sums[w] * __builtin_amdgcn_exp2f((maxima[w] - from) * scale);
+        }
+        if (on && t == 0) {
+            const int64_t token = token_of(a, r);
+            float y = 0.0f;
+            if (token >= a.cols) y = __builtin_nanf("");
+            else if (token >= 0) y = s == 0.0f ? -INF : ((float)row[token] - top) * inverse - logf(s);
+            a.logprobs[r] = y;
+            if (a.stats) {
+                a.stats[2 * r] = top;
+                a.stats[2 * r + 1] = s;
+            }
+        }
+    }
+}
+
+template <class T>
+__global__ __launch_bounds__(256) void logprobs_grad_kernel(Logprobs a, int slices) {
+    constexpr int N = Pack<T>::N, EACH = 2 * N;
+    for (int64_t w = blockIdx.x; w < a.rows * slices; w += gridDim.x) {
+        const int64_t r = w / slices;
+        const int64_t token = token_of(a, r);
+        const float temperature = a.temperature ? a.temperature[r] : 1.0f;
+        const float inverse = 1.0f / temperature, scale = inverse * LOG2E;
+        const float top = a.stats[2 * r], s = a.stats[2 * r + 1];
+        const bool scored = token >= 0 && s != 0.0f;
+        const float g = scored ? a.grad[r] * inverse : 0.0f;
+        const float less = token >= a.cols ? __builtin_nanf("") : g / s;
+        const T *row = row_of<T>(a.logits, r, a.inner);
+        T *out = row_of<T>(a.grad_logits, r, a.inner);
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+            const int col = (int)(w % slices) * 256 * EACH + (c * 256 + (int)threadIdx.x) * N;
+            if (col >= a.cols) continue;
+            float z[N];
+            load_floats<T, N>(row, col, a.cols, 0.0f, z);
+#pragma unroll
+            for (int e = 0; e < N; e++) {
+                const float d = scored ? -less * __builtin_amdgcn_exp2f((z[e] - top) * scale) : 0.0f;
+                z[e] = col + e == token ? g + d : d;
+            }
+            store_floats<T, N>(out, col, a.cols, z);
+        }
+    }
+}
+
+// ---- launches -----------------------------------------------------------------------------------------------------------
+
+// The caller's device for the launch, and what was current before it.
+struct OnDevice {
+    int was = -1;
+    bool moved = false;
+    zbpe_status go(int device) {
+        if (hipGetDevice(&was) != hipSuccess) return refuse(ZBPE_DEVICE_ERROR, "no HIP device");
+        if (was == device) return ZBPE_OK;
+        const hipError_t e = hipSetDevice(device);
+        if (e != hipSuccess) return refuse(ZBPE_DEVICE_ERROR, "device %d: %s", device, hipGetErrorString(e));
+        moved = true;
+        return ZBPE_OK;
+    }
+    ~OnDevice() {
+        if (moved) (void)hipSetDevice(was);
+    }
+};
+
+static zbpe_status launched(const char *what) {
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? ZBPE_OK : refuse(ZBPE_DEVICE_ERROR, "%s: %s", what, hipGetErrorString(e));
+}
+
+// Workgroups of a launch over `items`: each goes on by the grid's size, so any number of items is covered.
+static unsigned grid_of(int64_t items) { return (unsigned)(items < (1 << 21) ? items : (1 << 21)); }
+
+static bool is_float(int dtype) { return dtype == ZBPE_F32 || dtype == ZBPE_F16 || dtype == ZBPE_BF16; }
+static Rows rows_of(const zbpe_rows &m) { return Rows{(char *)m.data, m.outer_stride, m.inner_stride}; }
+
+static zbpe_status check_rows(const char *what, int64_t rows, int64_t inner, int cols) {
+    if (cols < 1 || cols > ZBPE_MAX_VOCAB) return refuse(ZBPE_INVALID_ARGUMENT, "%s: %d columns (1 to %d)", what, cols, ZBPE_MAX_VOCAB);
+    if (rows < 0 || rows >= (1ll << 40)) return refuse(ZBPE_INVALID_ARGUMENT, "%s: %lld rows", what, (long long)rows);
+    if (inner < 1) return refuse(ZBPE_INVALID_ARGUMENT, "%s: inner is %lld", what, (long long)inner);
+    return ZBPE_OK;
+}
+static zbpe_status check_matrix(const char *what, const char *name, const zbpe_rows &m, int64_t rows) {
+    if (!is_float(m.dtype)) return refuse(ZBPE_INVALID_ARGUMENT, "%s: %s has data type %d (F32, F16 or BF16)", what, name, m.dtype);
+    if (!m.data && rows) return refuse(ZBPE_INVALID_ARGUMENT, "%s: no %s", what, name);
+    return ZBPE_OK;
+}
+// rows that are written: none of them overlaps another
+static zbpe_status check_written(const char *what, const char *name, const zbpe_rows &m, int64_t rows, int64_t inner, int cols) {
+    const zbpe_status s = check_matrix(what, name, m, rows);
+    if (s != ZBPE_OK) return s;
+    const int64_t n_inner = rows < inner ? rows : inner, n_outer = rows / inner + (rows % inner != 0);
+    int64_t a = m.inner_stride < 0 ? -m.inner_stride : m.inner_stride, b = m.outer_stride < 0 ? -m.outer_stride : m.outer_stride;
+    const bool ok = (n_inner < 2 || a >= cols) && (n_outer < 2 || b >= cols) &&
+                    (n_inner < 2 || n_outer < 2 || b >= a * (n_inner - 1) + cols || a >= b * (n_outer - 1) + cols);
+    return ok ? ZBPE_OK : refuse(ZBPE_INVALID_ARGUMENT, "%s: the rows of %s overlap", what, name);
+}
+
+template <class F>
+static zbpe_status by_type(int dtype, F f) {
+    return dtype == ZBPE_F32 ? f(float()) : dtype == ZBPE_F16 ? f(f16()) : f(bf16());
+}
+
+static zbpe_status grammar_of(const char *what, const zbpe_grammar *g, int64_t rows, Automaton *out) {
+    if (!g) return refuse(ZBPE_INVALID_ARGUMENT, "%s: no grammar", what);
+    if (g->vocab_size < 1 || g->vocab_size > ZBPE_MAX_VOCAB)
+        return refuse(ZBPE_INVALID_ARGUMENT, "%s: a vocabulary of %d (1 to %d)", what, g->vocab_size, ZBPE_MAX_VOCAB);
+    if (g->end_token < -1 || g->end_token >= g->vocab_size) return refuse(ZBPE_INVALID_ARGUMENT, "%s: end token %d", what, g->end_token);
+    if (g->n_states < 0 || g->n_states >= (1 << 23)) return refuse(ZBPE_INVALID_ARGUMENT, "%s: %d states (fewer than 2^23)", what, g->n_states);
+    if (rows < 0 || rows >= (1ll << 40)) return refuse(ZBPE_INVALID_ARGUMENT, "%s: %lld rows", what, (long long)rows);
+    if (!g->offsets || !g->bytes || (!g->next && g->n_states)) return refuse(ZBPE_INVALID_ARGUMENT, "%s: an array of the grammar is missing", what);
+    *out = Automaton{g->offsets, g->bytes, g->next, g->accepting, g->vocab_size, g->end_token, g->n_states};
+    return ZBPE_OK;
+}
+
+static zbpe_status adjust_of(const char *what, const zbpe_adjust *p, Adjust *out) {
+    if (!p) return refuse(ZBPE_INVALID_ARGUMENT, "%s: no arguments", what);
+    if (p->struct_size != sizeof(zbpe_adjust)) return refuse(ZBPE_INVALID_ARGUMENT, "%s: arguments of another version", what);
+    zbpe_status s = check_rows(what, p->rows, p->inner, p->cols);
+    if (s == ZBPE_OK) s = check_matrix(what, "logits", p->logits, p->rows);
+    if (s != ZBPE_OK) return s;
+    if (p->out.dtype != p->logits.dtype && p->out.dtype != ZBPE_F32)
+        return refuse(ZBPE_INVALID_ARGUMENT, "%s: out has the type of the logits, or F32", what);
+    if (p->history_len < 0 || (p->history.data && p->history.dtype != ZBPE_I32 && p->history.dtype != ZBPE_I64))
+        return refuse(ZBPE_INVALID_ARGUMENT, "%s: a history of %lld tokens of data type %d (I32 or I64)", what, (long long)p->history_len, p->history.dtype);
+    if (p->history_len >= (1ll << 31)) return refuse(ZBPE_INVALID_ARGUMENT, "%s: a history of 2^31 tokens or more", what);
+    if (p->n_biases < 0 || p->n_biases > ZBPE_MAX_BIASES) return refuse(ZBPE_INVALID_ARGUMENT, "%s: %d biases (0 to %d)", what, p->n_biases, ZBPE_MAX_BIASES);
+    if (p->n_biases && p->rows && (!p->bias_tokens || !p->bias_values)) return refuse(ZBPE_INVALID_ARGUMENT, "%s: bias tokens without values, or values without tokens", what);
+    if (p->masks) {
+        if (p->mask_words < (p->cols + 31) / 32) return refuse(ZBPE_INVALID_ARGUMENT, "%s: %d words of mask for %d columns", what, p->mask_words, p->cols);
+        if (p->mask_rows < 0 || (!p->states && p->mask_rows != 1 && p->mask_rows < p->rows))
+            return refuse(ZBPE_INVALID_ARGUMENT, "%s: %lld rows of masks for %lld rows", what, (long long)p->mask_rows, (long long)p->rows);
+    }
+    Adjust a{};
+    a.logits = rows_of(p->logits);
+    a.out = rows_of(p->out);
+    if (p->history_len) a.history = rows_of(p->history);
+    a.wide_ids = p->history.dtype == ZBPE_I64;
+    a.rows = p->rows;
+    a.inner = p->inner;
+    a.cols = p->cols;
+    a.slices = (p->cols + ADJUST_SLICE - 1) / ADJUST_SLICE;
+    a.history_len = p->history_len;
+    a.lengths = p->lengths;
+    a.prompt_lengths = p->prompt_lengths;
+    a.repetition = p->repetition;
+    a.presence = p->presence;
+    a.frequency = p->frequency;
+    a.bias = p->bias;
+    a.bias_tokens = p->bias_tokens;
+    a.bias_values = p->bias_values;
+    a.n_biases = p->n_biases;
+    a.masks = p->masks;
+    a.words = p->mask_words;
+    a.mask_rows = p->mask_rows;
+    a.states = p->states;
+    *out = a;
+    return ZBPE_OK;
+}
+
+// Rows of one workgroup of the gradient: its columns' sums are kept over them, so more rows mean fewer partial sums to
+// write and add; fewer rows mean more workgroups. Up to 32, as long as four workgroups remain for each of the 256 CUs.
+static int adjust_run(int64_t rows, int cols) {
+    const int64_t slices = (cols + ADJUST_SLICE - 1) / ADJUST_SLICE, fit = rows * slices / 1024;
+    return (int)(fit < 1 ? 1 : fit > 32 ? 32 : fit);
+}
+static int64_t adjust_runs(int64_t rows, int cols) {
+    const int run = adjust_run(rows, cols);
+    return (rows + run - 1) / run;
+}
+
+template <class T>
+static void draw_launch(const Draw &a, hipStream_t stream) {
+    const dim3 grid(grid_of(a.rows));
+    if (a.cols <= 2048) draw_kernel<T, 256, 8><<<grid, 256, 0, stream>>>(a);
+    else if (a.cols <= 8192) draw_kernel<T, 512, 16><<<grid, 512, 0, stream>>>(a);
+    else if (a.cols <= 32768) draw_kernel<T, 1024, 32><<<grid, 1024, 0, stream>>>(a);
+    else draw_kernel<T, 1024, 64><<<grid, 1024, 0, stream>>>(a);
+}
+
+static zbpe_status logprobs_of(const char *what, const zbpe_logprobs *p, Logprobs *out) {
+    if (!p) return refuse(ZBPE_INVALID_ARGUMENT, "%s: no arguments", what);
+    if (p->struct_size != sizeof(zbpe_logprobs)) return refuse(ZBPE_INVALID_ARGUMENT, "%s: arguments of another version", what);
+    zbpe_status s = check_rows(what, p->rows, p->inner, p->cols);
+    if (s == ZBPE_OK) s = check_matrix(what, "logits", p->logits, p->rows);
+    if (s != ZBPE_OK) return s;
+    if (p->tokens_dtype != ZBPE_I32 && p->tokens_dtype != ZBPE_I64)
+        return refuse(ZBPE_INVALID_ARGUMENT, "%s: tokens of data type %d (I32 or I64)", what, p->tokens_dtype);
+    if (!p->tokens && p->rows) return refuse(ZBPE_INVALID_ARGUMENT, "%s: no tokens", what);
+    *out = Logprobs{rows_of(p->logits), {}, p->rows, p->inner, p->cols, p->tokens_dtype == ZBPE_I64, p->tokens, p->temperature, nullptr, p->logprobs, p->stats};
+    return ZBPE_OK;
+}
+
+}  // namespace zbpe
+
+using namespace zbpe;
+
+extern "C" {
+
+size_t zbpe_struct_size(int which) {
+    return which == 0 ? sizeof(zbpe_adjust) : which == 1 ? sizeof(zbpe_draw) : which == 2 ? sizeof(zbpe_logprobs) : which == 3 ? sizeof(zbpe_grammar) : 0;
+}
+
+zbpe_status zbpe_vocab_bytes(const uint16_t *triples, size_t n_merges, size_t vocab_size, uint32_t *offsets, uint8_t *bytes,
+                             size_t cap, size_t *n_bytes) {
+    if ((!triples && n_merges) || !offsets || !n_bytes || (!bytes && cap)) return refuse(ZBPE_INVALID_ARGUMENT, "zbpe_vocab_bytes: an array is missing");
+    if (vocab_size < 256 || vocab_size > ZBPE_MAX_VOCAB)
+        return refuse(ZBPE_INVALID_ARGUMENT, "zbpe_vocab_bytes: a vocabulary of %zu (256 to %d)", vocab_size, ZBPE_MAX_VOCAB);
+    try {
+        VocabTree tree;
+        const zbpe_status s = tree.build(triples, n_merges, vocab_size);
+        if (s != ZBPE_OK) return refuse(s, "zbpe_vocab_bytes: %s", tree.err.c_str());
+        *n_bytes = (size_t)tree.total;
+        tree.write(offsets, cap >= tree.total ? bytes : nullptr);
+        return ZBPE_OK;
+    } catch (const std::bad_alloc &) {
+        return refuse(ZBPE_OUT_OF_MEMORY, "zbpe_vocab_bytes: out of host memory");
+    } catch (const std::exception &e) {
+        return refuse(ZBPE_INTERNAL, "zbpe_vocab_bytes: %s", e.what());
+    }
+}
+
+zbpe_status zbpe_grammar_masks(int device, void *stream, const zbpe_grammar *grammar, const int32_t *states, int64_t rows,
+                               uint32_t *masks) {
+    const char *what = "zbpe_grammar_masks";
+    Automaton g;
+    zbpe_status s = grammar_of(what, grammar, rows, &g);
+    if (s != ZBPE_OK || !rows) return s;
+    if (!masks) return refuse(ZBPE_INVALID_ARGUMENT, "%s: no masks", what);
+    OnDevice on;
+    if ((s = on.go(device)) != ZBPE_OK) return s;
+    const int slices = (g.vocab + 255) / 256;
+    grammar_masks_kernel<<<grid_of(rows * slices), 256, 0, (hipStream_t)stream>>>(g, states, rows, masks, slices);
+    return launched(what);
+}
+
+zbpe_status zbpe_grammar_advance(int device, void *stream, const zbpe_grammar *grammar, const int32_t *states,
+                                 const int32_t *tokens, int64_t rows, int32_t *out) {
+    const char *what = "zbpe_grammar_advance";
+    Automaton g;
+    zbpe_status s = grammar_of(what, grammar, rows, &g);
+    if (s != ZBPE_OK || !rows) return s;
+    if (!states || !tokens || !out) return refuse(ZBPE_INVALID_ARGUMENT, "%s: an array is missing", what);
+    OnDevice on;
+    if ((s = on.go(device)) != ZBPE_OK) return s;
+    grammar_advance_kernel<<<grid_of((rows + 255) / 256), 256, 0, (hipStream_t)stream>>>(g, states, tokens, rows, out);
+    return launched(what);
+}
+
+zbpe_status zbpe_adjust_logits(int device, void *stream, const zbpe_adjust *args) {
+    const char *what = "zbpe_adjust_logits";
+    Adjust a;
+    zbpe_status s = adjust_of(what, args, &a);
+    if (s == ZBPE_OK) s = check_written(what, "out", args->out, a.rows, a.inner, a.cols);
+    if (s != ZBPE_OK || !a.rows) return s;
+    OnDevice on;
+    if ((s = on.go(device)) != ZBPE_OK) return s;
+    const unsigned grid = grid_of(a.rows * a.slices);
+    return by_type(args->logits.dtype, [&](auto ti) {
+        using T = decltype(ti);
+        if (args->out.dtype == ZBPE_F32) adjust_kernel<T, float><<<grid, ADJUST_THREADS, 0, (hipStream_t)stream>>>(a);
+        else adjust_kernel<T, T><<<grid, ADJUST_THREADS, 0, (hipStream_t)stream>>>(a);
+        return launched(what);
+    });
+}
+
+size_t zbpe_adjust_workspace(int64_t rows, int32_t cols) {
+    return rows < 1 || cols < 1 || cols > ZBPE_MAX_VOCAB ? 0 : (size_t)adjust_runs(rows, cols) * (size_t)cols * sizeof(float);
+}
+
+zbpe_status zbpe_adjust_logits_grad(int device, void *stream, const zbpe_adjust *args, const zbpe_rows *grad_logits,
+                                    float *grad_bias, float *grad_bias_values, void *workspace, size_t workspace_size) {
+    const char *what = "zbpe_adjust_logits_grad";
+    AdjustGrad g{};
+    zbpe_status s = adjust_of(what, args, &g.a);
+    if (s == ZBPE_OK) s = check_matrix(what, "the output's gradient", args->out, g.a.rows);
+    if (s == ZBPE_OK && grad_logits) {
+        if (grad_logits->dtype != args->logits.dtype) return refuse(ZBPE_INVALID_ARGUMENT, "%s: grad_logits has the type of the logits", what);
+        s = check_written(what, "grad_logits", *grad_logits, g.a.rows, g.a.inner, g.a.cols);
+        g.grad_logits = rows_of(*grad_logits);
+    }
+    if (s != ZBPE_OK) return s;
+    if (grad_bias && workspace_size < zbpe_adjust_workspace(g.a.rows, g.a.cols))
+        return refuse(ZBPE_INVALID_ARGUMENT, "%s: a workspace of %zu bytes, %zu are needed", what, workspace_size, zbpe_adjust_workspace(g.a.rows, g.a.cols));
+    if (grad_bias && !workspace && g.a.rows) return refuse(ZBPE_INVALID_ARGUMENT, "%s: no workspace", what);
+    OnDevice on;
+    if ((s = on.go(device)) != ZBPE_OK) return s;
+    g.grad_bias_values = g.a.n_biases ? grad_bias_values : nullptr;
+    g.sums = grad_bias ? (float *)workspace : nullptr;
+    g.run = adjust_run(g.a.rows, g.a.cols);
+    g.runs = (int)adjust_runs(g.a.rows, g.a.cols);
+    if (g.a.rows && (grad_logits || grad_bias || g.grad_bias_values)) {
+        const unsigned grid = grid_of((int64_t)g.runs * g.a.slices);
+        s = by_type(args->logits.dtype, [&](auto ti) {
+            using T = decltype(ti);
+            if (args->out.dtype == ZBPE_F32) adjust_grad_kernel<T, float><<<grid, ADJUST_THREADS, 0, (hipStream_t)stream>>>(g);
+            else adjust_grad_kernel<T, T><<<grid, ADJUST_THREADS, 0, (hipStream_t)stream>>>(g);
+            return launched(what);
+        });
+        if (s != ZBPE_OK) return s;
+    }
+    if (!grad_bias) return ZBPE_OK;
+    adjust_bias_kernel<<<(unsigned)(g.a.cols + 63) / 64, 256, 0, (hipStream_t)stream>>>(g.sums, g.runs, g.a.cols, grad_bias);
+    return launched(what);
+}
+
+zbpe_status zbpe_draw_tokens(int device, void *stream, const zbpe_draw *p) {
+    const char *what = "zbpe_draw_tokens";
+    if (!p) return refuse(ZBPE_INVALID_ARGUMENT, "%s: no arguments", what);
+    if (p->struct_size != sizeof(zbpe_draw)) return refuse(ZBPE_INVALID_ARGUMENT, "%s: arguments of another version", what);
+    zbpe_status s = check_rows(what, p->rows, p->inner, p->cols);
+    if (s == ZBPE_OK) s = check_matrix(what, "logits", p->logits, p->rows);
+    if (s != ZBPE_OK || !p->rows) return s;
+    if (!p->uniforms || !p->tokens) return refuse(ZBPE_INVALID_ARGUMENT, "%s: no uniforms, or no tokens", what);
+    OnDevice on;
+    if ((s = on.go(device)) != ZBPE_OK) return s;
+    const Draw a{rows_of(p->logits), p->rows, p->inner, p->cols, p->uniforms, p->temperature, p->top_p, p->min_p, p->top_k, p->tokens, p->logprobs};
+    return by_type(p->logits.dtype, [&](auto ti) {
+        draw_launch<decltype(ti)>(a, (hipStream_t)stream);
+        return launched(what);
+    });
+}
+
+zbpe_status zbpe_token_logprobs(int device, void *stream, const zbpe_logprobs *args) {
+    const char *what = "zbpe_token_logprobs";
+    Logprobs a;
+    zbpe_status s = logprobs_of(what, args, &a);
+    if (s != ZBPE_OK || !a.rows) return s;
+    if (!a.logprobs) return refuse(ZBPE_INVALID_ARGUMENT, "%s: no logprobs", what);
+    OnDevice on;
+    if ((s = on.go(device)) != ZBPE_OK) return s;
+    return by_type(args->logits.dtype, [&](auto ti) {
+        using T = decltype(ti);
+        if (a.cols <= 2048) logprobs_kernel<T, 64><<<grid_of((a.rows + 3) / 4), 256, 0, (hipStream_t)stream>>>(a);
+        else logprobs_kernel<T, 256><<<grid_of(a.rows), 256, 0, (hipStream_t)stream>>>(a);
+        return launched(what);
+    });
+}
+
+zbpe_status zbpe_token_logprobs_grad(int device, void *stream, const zbpe_logprobs *args, const float *grad,
+                                     const zbpe_rows *grad_logits) {
+    const char *what = "zbpe_token_logprobs_grad";
+    Logprobs a;
+    zbpe_status s = logprobs_of(what, args, &a);
+    if (s != ZBPE_OK) return s;
+    if (!grad_logits || grad_logits->dtype != args->logits.dtype) return refuse(ZBPE_INVALID_ARGUMENT, "%s: grad_logits has the type of the logits", what);
+    if ((s = check_written(what, "grad_logits", *grad_logits, a.rows, a.inner, a.cols)) != ZBPE_OK || !a.rows) return s;
+    if (!grad || !a.stats) return refuse(ZBPE_INVALID_ARGUMENT, "%s: no gradient, or no stats", what);
+    a.grad = grad;
+    a.grad_logits = rows_of(*grad_logits);
+    OnDevice on;
+    if ((s = on.go(device)) != ZBPE_OK) return s;
+    return by_type(args->logits.dtype, [&](auto ti) {
+        using T = decltype(ti);
+        const int each = 512 * Pack<T>::N, slices = (a.cols + each - 1) / each;
+        logprobs_grad_kernel<T><<<grid_of(a.rows * slices), 256, 0, (hipStream_t)stream>>>(a, slices);
+        return launched(what);
+    });
+}
+
+}  // extern "C"

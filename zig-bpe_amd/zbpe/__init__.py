@@ -153,6 +153,8 @@ EXPORTS = (
     "zbpe_train", "zbpe_upload", "zbpe_train_resident", "zbpe_encode", "zbpe_verify_counts", "zbpe_tokens",
     "zbpe_set_option", "zbpe_format_time_stats", "zbpe_bench_scan", "zbpe_bench_train_scan", "zbpe_merge_log", "zbpe_trace", "zbpe_scan_log", "zbpe_compaction_log", "zbpe_halt_log", "zbpe_zig_order_winner", "zbpe_version",
     "zbpe_stats_size", "zbpe_bench_recount",
+    "zbpe_vocab_bytes", "zbpe_grammar_masks", "zbpe_grammar_advance", "zbpe_adjust_logits", "zbpe_adjust_workspace",
+    "zbpe_adjust_logits_grad", "zbpe_draw_tokens", "zbpe_token_logprobs", "zbpe_token_logprobs_grad", "zbpe_struct_size",
 )
 MERGE_LOG_COLUMNS = ("key", "count", "live", "ties", "list_scan", "list_len", "key_live", "range")
 TRACE_COLUMNS = ("merge", "count", "live", "slots", "streamed", "scan_ms", "replace_ms", "select_ms", "wall_ms",
@@ -234,9 +236,21 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
     L.zbpe_halt_log.argtypes = [vp, vp, sz, ctypes.POINTER(sz)]
     L.zbpe_zig_order_winner.argtypes = [vp, vp, vp, sz, ctypes.c_uint32, ctypes.c_int, ctypes.POINTER(ctypes.c_uint32)]
     L.zbpe_version.restype = ctypes.c_char_p
+    if hasattr(L, "zbpe_draw_tokens"):  # (structures go as packed bytes: zbpe/logits.py)
+        i, i64 = ctypes.c_int, ctypes.c_int64
+        L.zbpe_vocab_bytes.argtypes = [vp, sz, sz, vp, vp, sz, ctypes.POINTER(sz)]
+        L.zbpe_grammar_masks.argtypes = [i, vp, vp, vp, i64, vp]
+        L.zbpe_grammar_advance.argtypes = [i, vp, vp, vp, vp, i64, vp]
+        L.zbpe_adjust_logits.argtypes = [i, vp, vp]
+        L.zbpe_adjust_workspace.argtypes = [i64, ctypes.c_int32]
+        L.zbpe_adjust_logits_grad.argtypes = [i, vp, vp, vp, vp, vp, vp, sz]
+        L.zbpe_draw_tokens.argtypes = [i, vp, vp]
+        L.zbpe_token_logprobs.argtypes = [i, vp, vp]
+        L.zbpe_token_logprobs_grad.argtypes = [i, vp, vp, vp, vp]
+        L.zbpe_struct_size.argtypes = [i]
     for name in EXPORTS:
         if name not in ("zbpe_destroy", "zbpe_last_error", "zbpe_version", "zbpe_stats_size") and hasattr(L, name):
-            getattr(L, name).restype = ctypes.c_int
+            getattr(L, name).restype = ctypes.c_size_t if name in ("zbpe_adjust_workspace", "zbpe_struct_size") else ctypes.c_int
     if hasattr(L, "zbpe_stats_size"):  # the caller-allocated zbpe_stats must match the library's layout
         L.zbpe_stats_size.restype = ctypes.c_size_t
         if L.zbpe_stats_size() != ctypes.sizeof(Stats):
@@ -613,6 +627,42 @@ class BasicTokenizer:
                 expand(m)
         return bytes(out)
 
+    # between a model's logits over this vocabulary and its tokens (no counterpart in the reference; zbpe/logits.py)
+
+    def vocabulary(self, vocabSize: Optional[int] = None, endToken: Optional[int] = None):
+        """The tokens of the merges as they are now, laid out on this tokenizer's device: logits.Vocabulary."""
+        from . import logits
+
+        return logits.Vocabulary(self.merges, vocabSize, endToken, f"cuda:{self._device}")
+
+    def grammar(self, next, accepting=None, vocabSize: Optional[int] = None, endToken: Optional[int] = None):
+        """An automaton over bytes, read by this vocabulary's tokens: logits.Grammar."""
+        from . import logits
+
+        return logits.Grammar(self.vocabulary(vocabSize, endToken), next, accepting)
+
+    def nextTokens(self, logits, uniforms, *, grammar=None, states=None, temperature=None, top_k=None, top_p=None,
+                   min_p=None, **terms):
+        """One decoding step of a batch: (tokens, log-probabilities, states after them). With a grammar, its masks for `states`
+        (int32, one a row) are made and applied; `terms` are adjust_logits' other arguments. A row that no token can follow
+        draws -1 and keeps its state. Without a grammar the third result is None."""
+        from . import logits as ops
+
+        if (grammar is None) != (states is None):
+            raise InvalidArgument("a grammar goes with states")
+        if grammar is not None:
+            if "masks" in terms:
+                raise InvalidArgument("masks and a grammar: give one")
+            terms["masks"] = grammar.masks(states)
+        if terms:
+            logits = ops.adjust_logits(logits.detach(), **terms)
+        tokens, logprobs = ops.draw_tokens(logits, uniforms, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+        return tokens, logprobs, None if grammar is None else grammar.advance(states, tokens)
+
+    def bitsPerByte(self, logits, tokens):
+        """What a model pays for a text in this vocabulary, in bits a byte: logits.Vocabulary.bits_per_byte."""
+        return self.vocabulary(vocabSize=max(logits.shape[-1], vocabStart)).bits_per_byte(logits, tokens)
+
     # serializeMerges (:319-330)
     def serializeMerges(self, file_path: str) -> None:
         with open(file_path, "wb") as f:
@@ -649,9 +699,21 @@ def merges_to_text(merges: np.ndarray) -> bytes:
     return "".join(f"{int(a)},{int(b)},{int(c)}\n" for a, b, c in np.asarray(merges).reshape(-1, 3)).encode()
 
 
+_LOGITS = ("Vocabulary", "Grammar", "adjust_logits", "draw_tokens", "token_logprobs", "token_bytes")
+
+
+def __getattr__(name: str):
+    if name in _LOGITS:  # (loaded when asked for: they need torch, the tokenizer does not)
+        from . import logits
+
+        return getattr(logits, name)
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+
+
 __all__ = [
     "BasicTokenizer", "CharPair", "Merge", "Merges", "Engine", "Stats", "TrainError", "InvalidVocabSize", "InvalidUtf8",
     "OutOfMemory", "DeviceError", "InvalidToken", "InvalidFormat", "InvalidCharacter", "Overflow", "StreamTooLong",
     "InvalidArgument", "InternalError", "load_library", "synth_corpus", "comm_unique_id", "zig_order_winner",
     "merges_to_text", "format_time_stats", "vocabStart", "EXPORTS", "TRACE_COLUMNS", "torch_collective", "COLLECTIVE_FN",
+    "Vocabulary", "Grammar", "adjust_logits", "draw_tokens", "token_logprobs", "token_bytes",
 ]
