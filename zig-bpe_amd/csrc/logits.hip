@@ -388,232 +388,473 @@ __device__ __forceinline__ uint32_t key_of(float z) {
 }
 __device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
 
-// One workgroup keeps a row in registers (NE values a thread) and goes over it as often as the filters need.
-template <class T, int NT, int NE>
-struct Drawer {
-    static constexpr int N = Pack<T>::N, C = NE / N, W = NT / 64, SEGMENTS = C * W;
-    struct Shared {
-        uint64_t start[SEGMENTS];  // the sum of the weights in front of each segment (chunk c of wave w: c * W + w, in id order)
-        uint64_t mass[256];
-        uint64_t total, base;
-        float maxima[W];
-        int col, bin;
-    };
-    float z[NE];
-    Shared &sh;
-    int cols;
-    float top;         // the row's maximum
-    double inverse;    // 1 / temperature
-    uint32_t cut_key;  // kept: a larger key, or this one up to cut_col
-    int cut_col;
+// A value and its column as one number, larger for an earlier rank (a larger value, then a smaller column). 0: none.
+__device__ __forceinline__ uint64_t pair_of(float z, int col) { return (uint64_t)key_of(z) << 32 | (uint32_t)~col; }
+__device__ __forceinline__ float value_of(uint64_t pair) { return of_key((uint32_t)(pair >> 32)); }
+__device__ __forceinline__ int col_of(uint64_t pair) { return (int)~(uint32_t)pair; }
 
-    __device__ __forceinline__ static int col_of(int c, int e) { return (c * NT + (int)threadIdx.x) * N + e; }
-    __device__ __forceinline__ bool kept(float v, int col) const {
-        const uint32_t k = key_of(v);
-        return v > -INF && (k > cut_key || (k == cut_key && col <= cut_col));
+// The same in every lane of a wave: in scalar registers.
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); }
+__device__ __forceinline__ float uniform(float x) { return __uint_as_float(uniform(__float_as_uint(x))); }
+__device__ __forceinline__ uint64_t uniform(uint64_t x) {
+    return (uint64_t)uniform((uint32_t)(x >> 32)) << 32 | uniform((uint32_t)x);
+}
+__device__ __forceinline__ double uniform(double x) { return __longlong_as_double((int64_t)uniform((uint64_t)__double_as_longlong(x))); }
+
+// One workgroup draws from one row, which it reads as often as the filters need (the first time from memory, then from the
+// caches: 1000 rows of 65535 floats in 122 us, 2.1 TB/s; kept in registers instead, a row leaves no room for a second
+// workgroup on the CU, and 2.3 ms). The usual filters leave few tokens, and those are found without looking at every value
+// twice: with NT threads over interleaved columns, the k-th largest of the threads' maxima is no larger than the k-th largest
+// value, and little more than k values reach it. They go to one thread each, are sorted, cut, and drawn from. Only where more
+// than NT values would have to be looked at (a large k, a flat distribution) the cut is found by histograms over the row.
+// What bounds it: the exponentials of rows without top_k (about 25 operations of 64 bits for each value).
+template <class T, int NT>
+struct Drawer {
+    static constexpr int N = Pack<T>::N, W = NT / 64, AHEAD = 4, BINS = 1024;
+    struct Shared {
+        uint64_t bins[BINS];   // the histogram
+        uint64_t list[NT];     // gathered pairs
+        uint64_t sorted[NT];   // the same in order
+        uint32_t rank[NT];
+        double power[256];     // 2^(i / 256)
+        uint64_t part[W], low[W], high[W];
+        float maxima[W], minima[W];
+        int counts[2][W];
+        int count, bin, col;
+        uint64_t above, cut;
+    };
+    Shared &sh;
+    const T *row;
+    int cols;
+    float top;      // the row's maximum
+    float floor;    // values below it count for nothing
+    double scale;   // 256 log2(e) / temperature
+    uint64_t cut;   // kept: this pair and larger ones
+    bool ones;      // every kept value counts as 1
+    double least;   // of the kept values' weights
+
+    // A 64-bit constant in scalar registers, set where it is used: kept through a loop, these constants would push its own
+    // values out of the vector registers.
+    template <uint64_t BITS>
+    __device__ __forceinline__ static double constant() {
+        uint32_t low, high;
+        asm volatile("s_mov_b32 %0, %1" : "=s"(low) : "i"((uint32_t)BITS));
+        asm volatile("s_mov_b32 %0, %1" : "=s"(high) : "i"((uint32_t)(BITS >> 32)));
+        return __longlong_as_double((int64_t)((uint64_t)high << 32 | low));
     }
+    // ln of the weight in 1 / 256 of a doubling (not above 0: +inf is taken as the largest finite value)
+    __device__ __forceinline__ double place_of(float v) const {
+        return ((double)fminf(v, 0x1.fffffep127f) - (double)fminf(top, 0x1.fffffep127f)) * scale;
+    }
+    // exp((v - top) / temperature) = 2^(y / 256), y = n + f with |f| <= 1/2: a power of two, an entry of the table, and four
+    // terms of the series of 2^(f / 256), which end below 2^-54. For v >= floor: the power of two is added to the exponent.
     __device__ __forceinline__ double weight(float v) const {
-        return v == top ? 1.0 : top == INF ? 0.0 : exp(((double)v - (double)top) * inverse);
+        const double y = place_of(v), magic = constant<0x4338000000000000>();  // 1.5 * 2^52
+        const double shifted = y + magic;
+        const int n = (int)(uint32_t)__double_as_longlong(shifted);
+        const double f = y - (shifted - magic);
+        double q = fma(f, constant<0x3d83b2ab6fba4e77>(), constant<0x3e2c6b08d704a0c0>());  // (ln 2 / 256)^n / n!, n = 4, 3
+        q = fma(f, q, constant<0x3ecebfbdff82c58f>());                                      // 2
+        q = fma(f, q, constant<0x3f662e42fefa39ef>()) * f;                                  // 1
+        const double power = __longlong_as_double(__double_as_longlong(sh.power[n & 255]) + ((int64_t)(n >> 8) << 52));
+        return fma(power, q, power);
     }
     // 2^47 w rounded: w + 32 has steps of 2^-47, and its mantissa is the multiple
     __device__ __forceinline__ static uint64_t steps(double w) {
-        return (uint64_t)__double_as_longlong(w + 32.0) & ((1ull << 52) - 1);
+        return (uint64_t)__double_as_longlong(w + constant<0x4040000000000000>()) & ((1ull << 52) - 1);
     }
+    __device__ __forceinline__ uint64_t mass(float v) const {
+        const uint64_t x = steps(weight(v));
+        return v >= floor ? x : 0;
+    }
+    __device__ __forceinline__ uint64_t share(float v, int col) const {
+        if (!(v >= floor)) return 0;
+        if (cut && pair_of(v, col) < cut) return 0;
+        if (ones) return 1;
+        const double w = weight(v);
+        return w >= least ? steps(w) : 0;
+    }
+    // What is below the floor weighs nothing (under 2^-48): 36 temperatures down. (Rounding the floor moves it past no value.)
+    __device__ __forceinline__ float floor_of(float temperature) const {
+        return uniform(top == INF ? INF : fmaxf(top - 36.0f * temperature, -0x1.fffffep127f));
+    }
+    // NaN counts as -inf; one key for both zeros
+    __device__ __forceinline__ static float clean(float z) { return (z == z ? z : -INF) + 0.0f; }
 
-    __device__ __forceinline__ void load(const T *row) {
+    // f(value, column) over columns from + (t + i * step) * N .. + N, up to `to`; AHEAD packs are on their way at a time
+    template <int AHEAD, class F>
+    __device__ __forceinline__ void each(int t, int step, int from, int to, F f) {
+        int col = from + t * N;
+#pragma unroll 1
+        for (; col + ((AHEAD - 1) * step + 1) * N <= to; col += AHEAD * step * N) {
+            Pack<T> z[AHEAD];
 #pragma unroll
-        for (int c = 0; c < C; c++) load_floats<T, N>(row, col_of(c, 0), cols, -INF, z + c * N);
-        float m = -INF;
+            for (int a = 0; a < AHEAD; a++) z[a] = load_pack(row + col + a * step * N);
 #pragma unroll
-        for (int i = 0; i < NE; i++) {
-            z[i] = z[i] == z[i] ? z[i] + 0.0f : -INF;  // (+ 0: one key for both zeros)
-            m = fmaxf(m, z[i]);
+            for (int a = 0; a < AHEAD; a++)
+#pragma unroll
+                for (int e = 0; e < N; e++) f(clean((float)z[a].v[e]), col + a * step * N + e);
         }
-        m = wave_max(m);
-        if ((threadIdx.x & 63) == 0) sh.maxima[threadIdx.x >> 6] = m;
-        __syncthreads();
-        top = -INF;
+#pragma unroll 1
+        for (; col < to; col += step * N) {
+            float z[N];
+            load_floats<T, N>(row, col, to, -INF, z);
 #pragma unroll
-        for (int w = 0; w < W; w++) top = fmaxf(top, sh.maxima[w]);
-        cut_key = 0;
-        cut_col = 1 << 30;
+            for (int e = 0; e < N; e++)
+                if (col + e < to) f(clean(z[e]), col + e);
+        }
     }
-
-    // Sums f(value, column) over the row in id order; leaves the sums in front of each segment in `start`.
     template <class F>
-    __device__ __forceinline__ uint64_t total(F f) {
-        const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-        __syncthreads();
-#pragma unroll
-        for (int c = 0; c < C; c++) {
-            uint64_t s = 0;
-#pragma unroll
-            for (int e = 0; e < N; e++) s += f(z[c * N + e], col_of(c, e));
-            s = wave_sum(s);
-            if (lane == 0) sh.start[c * W + wave] = s;
-        }
-        __syncthreads();
-        if (wave == 0) {
-            constexpr int EACH = (SEGMENTS + 63) / 64;
-            uint64_t own[EACH], s = 0;
-#pragma unroll
-            for (int i = 0; i < EACH; i++) {
-                own[i] = lane * EACH + i < SEGMENTS ? sh.start[lane * EACH + i] : 0;
-                s += own[i];
-            }
-            uint64_t at = wave_scan(s) - s;
-#pragma unroll
-            for (int i = 0; i < EACH; i++) {
-                if (lane * EACH + i < SEGMENTS) sh.start[lane * EACH + i] = at;
-                at += own[i];
-            }
-            if (lane == 63) sh.total = at;
-        }
-        __syncthreads();
-        return sh.total;
+    __device__ __forceinline__ void each(F f) {  // the whole row, neighbouring packs by neighbouring threads
+        each<4>(threadIdx.x, NT, 0, cols, f);
     }
 
-    // After total(f): the first column at which the sum of f, that column included, exceeds t (t < the total).
-    template <class F>
-    __device__ __forceinline__ int locate(uint64_t t, F f) {
+    // The sum of x over the threads in front of this one; over all in `total`.
+    __device__ __forceinline__ uint64_t scan(uint64_t x, uint64_t &total) {
         const int wave = threadIdx.x >> 6;
-#pragma unroll
-        for (int c = 0; c < C; c++) {
-            const int seg = c * W + wave;
-            const uint64_t from = sh.start[seg], to = seg + 1 < SEGMENTS ? sh.start[seg + 1] : sh.total;
-            if (from <= t && t < to) {  // (one segment of one wave)
-                uint64_t s = 0;
-#pragma unroll
-                for (int e = 0; e < N; e++) s += f(z[c * N + e], col_of(c, e));
-                uint64_t at = from + wave_scan(s) - s;
-                if (at <= t && t < at + s) {
-                    bool open = true;
-#pragma unroll
-                    for (int e = 0; e < N; e++) {
-                        at += f(z[c * N + e], col_of(c, e));
-                        if (open && at > t) {
-                            open = false;
-                            sh.col = col_of(c, e);
-                        }
-                    }
-                }
-            }
-        }
+        const uint64_t in = wave_scan(x);
         __syncthreads();
-        return sh.col;
+        if ((threadIdx.x & 63) == 63) sh.part[wave] = in;
+        __syncthreads();
+        uint64_t at = in - x, all = 0;
+#pragma unroll 4
+        for (int w = 0; w < W; w++) {
+            if (w < wave) at += sh.part[w];
+            all += sh.part[w];
+        }
+        total = all;
+        return at;
     }
 
-    // Moves the cut to the last of the first ranks whose f sum to `target` or more (0 < target <= the sum over what is kept).
-    // f depends on the value alone. Eight bits of the key at a time.
-    template <class F>
-    __device__ __forceinline__ void cut_at(uint64_t target, F f) {
-        uint32_t found = 0;
+    // The n pairs of the threads (all different; 0: none), in order, larger first. Each is compared with all others, by NT / n
+    // threads: for the few pairs that are sorted here quicker than a network's many steps (1024 pairs: 20 us, 256: 2).
+    __device__ __forceinline__ uint64_t sort(uint64_t x, int n) {
+        const int t = threadIdx.x;
+        int width = 64;
+        while (width < n) width <<= 1;
+        const int parts = NT / width, each = (n + parts - 1) / parts;
+        __syncthreads();
+        sh.list[t] = x;
+        sh.rank[t] = 0;
+        sh.sorted[t] = 0;
+        __syncthreads();
+        const uint64_t mine = sh.list[t & (width - 1)];
+        const int from = t / width * each, to = from + each < n ? from + each : n;
+        uint32_t larger = 0;
+        int i = from;
+        for (; i + 4 <= to; i += 4)
+#pragma unroll
+            for (int e = 0; e < 4; e++) larger += sh.list[i + e] > mine;
+        for (; i < to; i++) larger += sh.list[i] > mine;
+        if (larger) atomicAdd(&sh.rank[t & (width - 1)], larger);
+        __syncthreads();
+        if (x) sh.sorted[sh.rank[t]] = x;
+        __syncthreads();
+        return sh.sorted[t];
+    }
+    // How many threads say so. Calls alternate between two places, so that one barrier a call is enough.
+    __device__ __forceinline__ int count(bool x, int turn) {
+        const int n = __popcll(__ballot(x));
+        if ((threadIdx.x & 63) == 0) sh.counts[turn & 1][threadIdx.x >> 6] = n;
+        __syncthreads();
+        int all = 0;
+#pragma unroll 4
+        for (int w = 0; w < W; w++) all += sh.counts[turn & 1][w];
+        return (int)uniform((uint32_t)all);
+    }
+
+    // Waves take the row in contiguous parts: their sums of the shares give the part that t falls into, and the pieces of that
+    // part, one for each wave, the place.
+    __device__ __forceinline__ int part_size() const { return (cols + W * 64 * N - 1) / (W * 64 * N) * (64 * N); }
+    __device__ __forceinline__ uint64_t part_sums() {
+        const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, size = part_size(), from = wave * size;
+        uint64_t s = 0, all = 0;
+        const int to = from + size < cols ? from + size : cols;
+        if (!cut && !ones && least == 0.0) each<1>(lane, 64, from, to, [&](float v, int) { s += mass(v); });
+        else each<1>(lane, 64, from, to, [&](float v, int col) { s += share(v, col); });
+        s = wave_sum(s);
+        __syncthreads();
+        if (lane == 0) sh.part[wave] = s;
+        __syncthreads();
+#pragma unroll 4
+        for (int w = 0; w < W; w++) all += sh.part[w];
+        return all;
+    }
+    // After part_sums: leaves in sh.col the first column at which the sum of shares, that column included, exceeds t (t < the total).
+    __device__ __forceinline__ void locate(uint64_t t) {
+        const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, size = part_size();
         uint64_t base = 0;
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            __syncthreads();
-            for (int i = threadIdx.x; i < 256; i += NT) sh.mass[i] = 0;
-            __syncthreads();
+        int part = 0;
+        while (t >= base + sh.part[part]) base += sh.part[part++];
+        const int from = part * size, to = from + size < cols ? from + size : cols;
+        // pieces of 64 * N columns, W at a time
+        for (int first = from; first < to; first += W * 64 * N) {
+            const int col = first + (wave * 64 + lane) * N;
+            uint64_t each[N], s = 0;
+            float z[N];
+            load_floats<T, N>(row, col, to, -INF, z);
 #pragma unroll
-            for (int i = 0; i < NE; i++) {
-                const uint32_t k = key_of(z[i]);
-                if (kept(z[i], col_of(i / N, i % N)) && (shift == 24 || k >> (shift + 8) == found))
-                    atomicAdd((unsigned long long *)&sh.mass[(k >> shift) & 255], (unsigned long long)f(z[i]));
-            }
-            __syncthreads();
-            if (threadIdx.x < 64) {
-                uint64_t own[4], s = 0;
+            for (int e = 0; e < N; e++) s += each[e] = share(clean(z[e]), col + e);
+            uint64_t all, at = base + scan(s, all);
+            if (at <= t && t < at + s) {
+                bool open = true;
 #pragma unroll
-                for (int i = 0; i < 4; i++) s += own[i] = sh.mass[255 - (4 * threadIdx.x + i)];
-                uint64_t at = base + wave_scan(s) - s;
-                if (at < target && target <= at + s) {
-                    bool open = true;
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        if (open && target <= at + own[i]) {
-                            open = false;
-                            sh.bin = 255 - (4 * (int)threadIdx.x + i);
-                            sh.base = at;
-                        }
-                        at += own[i];
+                for (int e = 0; e < N; e++) {
+                    at += each[e];
+                    if (open && at > t) {
+                        open = false;
+                        sh.col = col + e;
                     }
                 }
             }
-            __syncthreads();
-            found = found << 8 | (uint32_t)sh.bin;
-            base = sh.base;
+            base += all;
+            if (t < base) break;
         }
-        // of the values equal to the cut's, the first by id
-        const uint64_t each = f(of_key(found)), ties = (target - base + each - 1) / each;
-        auto tie = [&](float v, int col) -> uint64_t { return key_of(v) == found && kept(v, col) ? 1 : 0; };
-        total(tie);
-        const int col = locate(ties - 1, tie);
-        cut_key = found;
-        cut_col = col;
-    }
-};
-
-template <class T, int NT, int NE>
-__global__ __launch_bounds__(NT) void draw_kernel(Draw a) {
-    using D = Drawer<T, NT, NE>;
-    __shared__ typename D::Shared sh;
-    for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
         __syncthreads();
-        D d{{}, sh, a.cols, 0.0f, 0.0, 0u, 0};
-        d.load(row_of<T>(a.logits, r, a.inner));
-        const float temperature = a.temperature ? a.temperature[r] : 1.0f;
-        if (!(d.top > -INF)) {
+    }
+
+    // The pairs that `want` takes, one a thread in any order (0 past them); returns how many there are, which may be more
+    // than NT. `mine`: whether this thread's columns can hold any.
+    template <class F>
+    __device__ __forceinline__ int gather(bool mine, uint64_t &pair, F want) {
+        __syncthreads();
+        if (threadIdx.x == 0) sh.count = 0;
+        __syncthreads();
+        auto keep = [&](float v, int col) {
+            if (!want(v, col)) return;
+            const int i = atomicAdd(&sh.count, 1);
+            if (i < NT) sh.list[i] = pair_of(v, col);
+        };
+        if (mine) each<1>(threadIdx.x, NT, 0, cols, keep);
+        __syncthreads();
+        const int n = (int)uniform((uint32_t)sh.count);
+        pair = (int)threadIdx.x < n ? sh.list[threadIdx.x] : 0;
+        return n;
+    }
+
+    // Apart from the kernel, whose loops would pay for its registers.
+    __device__ __attribute__((noinline)) static uint64_t cut_apart(Shared &sh, const T *row, int cols, float top, float floor, double scale,
+                                                                   uint64_t cut, bool ones, uint64_t target, float temperature) {
+        Drawer d{sh, row, cols, uniform(top), uniform(floor), uniform(scale), uniform(cut), ones, 0.0};
+        d.cut_at(uniform(target), uniform(temperature));
+        return d.cut;
+    }
+    // Moves the cut to the last of the first ranks whose shares sum to `target` or more (0 < target <= the whole sum).
+    __device__ __forceinline__ void cut_at(uint64_t target, float temperature) {
+        // bins of equal width in value, down to where weights vanish; then within a bin, of equal numbers of pairs
+        const float width_inverse = (BINS - 1) / (40.0f * temperature);
+        uint64_t low = 0, high = ~0ull, above = 0;
+        int shift = -1;  // -1: by value
+        for (;;) {
+            auto bin_of = [&](float v, uint64_t pair) {
+                if (shift < 0) return v == top ? 0 : (int)fminf((top - v) * width_inverse, (float)(BINS - 1));
+                return (int)((high - pair) >> shift);
+            };
+            auto within = [&](float v, uint64_t pair) { return v > -INF && pair >= cut && pair >= low && pair <= high; };
+            __syncthreads();
+            for (int i = threadIdx.x; i < BINS; i += NT) sh.bins[i] = 0;
+            __syncthreads();
+            each([&](float v, int col) {
+                const uint64_t pair = pair_of(v, col);
+                if (within(v, pair)) atomicAdd((unsigned long long *)&sh.bins[bin_of(v, pair)], (unsigned long long)share(v, col));
+            });
+            __syncthreads();
+            constexpr int EACH = BINS / NT;
+            uint64_t own[EACH], s = 0, all;
+#pragma unroll
+            for (int i = 0; i < EACH; i++) s += own[i] = sh.bins[threadIdx.x * EACH + i];
+            uint64_t at = above + scan(s, all);
+            if (at < target && target <= at + s) {
+                bool open = true;
+#pragma unroll
+                for (int i = 0; i < EACH; i++) {
+                    if (open && target <= at + own[i]) {
+                        open = false;
+                        sh.bin = threadIdx.x * EACH + i;
+                        sh.above = at;
+                    }
+                    at += own[i];
+                }
+            }
+            __syncthreads();
+            const int bin = sh.bin;
+            above = sh.above;
+            // what is in that bin
+            uint64_t least_pair = ~0ull, most_pair = 0, pair;
+            const int n = gather(true, pair, [&](float v, int col) {
+                const uint64_t x = pair_of(v, col);
+                const bool in = within(v, x) && bin_of(v, x) == bin;
+                if (in) {
+                    least_pair = x < least_pair ? x : least_pair;
+                    most_pair = x > most_pair ? x : most_pair;
+                }
+                return in;
+            });
+            if (n <= NT) {
+                pair = sort(pair, n);
+                const uint64_t w = pair ? share(value_of(pair), col_of(pair)) : 0;
+                const uint64_t from = above + scan(w, all);
+                if (from < target && target <= from + w) sh.cut = pair;
+                __syncthreads();
+                cut = uniform(sh.cut);
+                return;
+            }
+            for (int d = 32; d; d >>= 1) {
+                const uint64_t x = __shfl_xor((unsigned long long)least_pair, d), y = __shfl_xor((unsigned long long)most_pair, d);
+                least_pair = x < least_pair ? x : least_pair;
+                most_pair = y > most_pair ? y : most_pair;
+            }
+            if ((threadIdx.x & 63) == 0) {
+                sh.low[threadIdx.x >> 6] = least_pair;
+                sh.high[threadIdx.x >> 6] = most_pair;
+            }
+            __syncthreads();
+            low = ~0ull;
+            high = 0;
+            for (int w = 0; w < W; w++) {
+                low = sh.low[w] < low ? sh.low[w] : low;
+                high = sh.high[w] > high ? sh.high[w] : high;
+            }
+            shift = 0;
+            while ((high - low) >> shift >= (uint64_t)BINS) shift++;
+        }
+    }
+
+    // Draws from the few pairs that can be left by the first k ranks (k > 0), or by the first that sum to `target`; false when
+    // that would be more than NT, or not enough.
+    __device__ __forceinline__ bool few(float mine, int k, float p, double least_kept, uint64_t target, uint64_t scaled, uint64_t &whole) {
+        // a threshold that `wanted` to 1.2 times as many threads' maxima reach
+        const int wanted = k > 0 ? k : NT / 4;
+        const uint32_t key = key_of(mine);
+        float least_mine = sh.minima[0];
+#pragma unroll 4
+        for (int w = 1; w < W; w++) least_mine = fminf(least_mine, sh.minima[w]);
+        uint32_t low = uniform(max(key_of(least_mine), key_of(-INF) + 1)), high = key_of(top);
+        for (int i = 0; i < 32 && low < high; i++) {
+            const uint32_t mid = low + (high - low) / 2 + 1;
+            const int n = count(key >= mid, i);
+            if (n < wanted) high = mid - 1;
+            else {
+                low = mid;
+                if (n <= wanted + wanted / 5) break;
+            }
+        }
+        uint64_t pair, all;
+        const int n = gather(key >= low, pair, [&](float v, int) { return key_of(v) >= low; });
+        if (n > NT) return false;
+        pair = sort(pair, n);
+        const bool in = pair && (k <= 0 || (int)threadIdx.x < k);
+        const bool weighs = in && value_of(pair) >= floor;
+        const double w = weighs ? weight(value_of(pair)) : 0.0;
+        const uint64_t at = scan(weighs ? steps(w) : 0, all);
+        if (k > 0) target = target_of(p, all);
+        else if (all < target) return false;
+        const bool keep = in && (p >= 1.0f || at < target) && w >= least_kept;
+        const int left = count(keep, 0);  // (they are the first ones)
+        const uint64_t by_id = sort(keep ? pair << 32 | pair >> 32 : 0, left);
+        const float v = of_key((uint32_t)by_id);
+        const uint64_t s = by_id ? mass(v) : 0;
+        const uint64_t from = scan(s, whole), t = __umul64hi(whole, scaled);
+        if (from <= t && t < from + s) sh.col = (int)~(uint32_t)(by_id >> 32);
+        __syncthreads();
+        return true;
+    }
+    __device__ __forceinline__ static uint64_t target_of(float p, uint64_t whole) {
+        const uint64_t t = (uint64_t)ceil((double)p * (double)whole);
+        return t < 1 ? 1 : t > whole ? whole : t;
+    }
+
+    __device__ __forceinline__ void draw(const Draw &a, int64_t r) {
+        const float temperature = a.temperature ? a.temperature[r] : 1.0f, p = a.top_p ? a.top_p[r] : 1.0f;
+        const float least_f = a.min_p ? a.min_p[r] : 0.0f, u = a.uniforms[r];
+        const int k = a.top_k ? a.top_k[r] : 0;
+        // the maximum of this thread's columns, and the first column that holds it
+        float mine = -INF;
+        int place = 0;
+        each([&](float v, int col) {
+            if (v > mine) {
+                mine = v;
+                place = col;
+            }
+        });
+        top = wave_max(mine);
+        const float lowest = -wave_max(-mine);
+        if ((threadIdx.x & 63) == 0) {
+            sh.maxima[threadIdx.x >> 6] = top;
+            sh.minima[threadIdx.x >> 6] = lowest;
+        }
+        if (threadIdx.x == 0) sh.col = cols;
+        __syncthreads();
+#pragma unroll 4
+        for (int w = 0; w < W; w++) top = fmaxf(top, sh.maxima[w]);
+        top = uniform(top);
+        if (!(top > -INF)) {
             if (threadIdx.x == 0) {
                 a.tokens[r] = -1;
                 if (a.logprobs) a.logprobs[r] = -INF;
             }
-            continue;
+            return;
         }
-        if (!(temperature > 0.0f)) {
-            auto first = [&](float v, int) -> uint64_t { return v == d.top ? 1 : 0; };
-            d.total(first);
-            const int col = d.locate(0, first);
+        if (!(temperature > 0.0f) || k == 1 || p <= 0.0f) {  // the first rank
+            if (mine == top) atomicMin(&sh.col, place);
+            __syncthreads();
             if (threadIdx.x == 0) {
-                a.tokens[r] = col;
+                a.tokens[r] = sh.col;
                 if (a.logprobs) a.logprobs[r] = 0.0f;
             }
-            continue;
+            return;
         }
-        d.inverse = 1.0 / (double)temperature;
-        auto one = [&](float v) -> uint64_t { return 1; };
-        auto mass = [&](float v) -> uint64_t { return d.steps(d.weight(v)); };
-        const int k = a.top_k ? a.top_k[r] : 0;
-        if (k > 0 && k < a.cols) {
-            const uint64_t n = d.total([&](float v, int col) -> uint64_t { return d.kept(v, col) ? 1 : 0; });
-            if ((uint64_t)k < n) d.cut_at((uint64_t)k, one);
-        }
-        const float p = a.top_p ? a.top_p[r] : 1.0f;
-        if (p < 1.0f) {
-            const uint64_t whole = d.total([&](float v, int col) -> uint64_t { return d.kept(v, col) ? mass(v) : 0; });
-            uint64_t target = p > 0.0f ? (uint64_t)ceil((double)p * (double)whole) : 1;
-            target = target < 1 ? 1 : target > whole ? whole : target;
-            d.cut_at(target, mass);
-        }
-        const float least_f = a.min_p ? a.min_p[r] : 0.0f;
-        const double least = least_f > 0.0f ? least_f < 1.0f ? (double)least_f : 1.0 : 0.0;
-        auto share = [&](float v, int col) -> uint64_t {
-            if (!d.kept(v, col)) return 0;
-            const double w = d.weight(v);
-            return w >= least ? d.steps(w) : 0;
-        };
-        const uint64_t whole = d.total(share);
+        scale = uniform(256 * 0x1.71547652b82fep0 / (double)temperature);
+        cut = 0;
+        const double least_kept = uniform(least_f > 0.0f ? least_f < 1.0f ? (double)least_f : 1.0 : 0.0);
         // u * whole without rounding: u < 1 is a multiple of 2^-64 here (24 bits), and the product's high half its floor
-        const float u = a.uniforms[r];
         const uint64_t scaled = u >= 1.0f ? ~0ull : u > 0.0f ? (uint64_t)((double)u * 18446744073709551616.0) : 0ull;
-        const int col = d.locate(__umul64hi(whole, scaled), share);
+        const bool by_k = k > 0 && k < cols, by_p = p < 1.0f;
+        bool untried = !by_k || k <= NT * 5 / 8;
+        uint64_t whole;
+        // 0: the cut by rank, 1: by share, 2: the draw from what is left
+        for (int stage = by_k ? 0 : by_p ? 1 : 2;;) {
+            ones = stage == 0;
+            floor = ones ? -0x1.fffffep127f : floor_of(temperature);
+            least = stage == 2 ? least_kept : 0.0;
+            const bool sums = stage || !untried;
+            if (sums) whole = uniform(part_sums());
+            if (stage == 2) {
+                locate(__umul64hi(whole, scaled));
+                break;
+            }
+            const uint64_t target = stage ? target_of(p, whole) : (uint64_t)k;
+            if (untried) {
+                untried = false;
+                uint64_t left;
+                floor = floor_of(temperature);
+                if (few(mine, by_k ? k : 0, p, least_kept, target, scaled, left)) {
+                    whole = left;
+                    break;
+                }
+                if (!sums) continue;
+            }
+            if (target < whole) cut = uniform(cut_apart(sh, row, cols, top, floor, scale, cut, ones, target, temperature));
+            stage = stage == 0 && by_p ? 1 : 2;
+        }
         if (threadIdx.x == 0) {
+            const int col = sh.col;
             a.tokens[r] = col;
             if (a.logprobs) {
-                const float v = (float)row_of<T>(a.logits, r, a.inner)[col];
-                const double x = v == d.top ? 0.0 : ((double)v - (double)d.top) * d.inverse;
+                const double x = place_of(clean((float)row[col])) * (0x1.62e42fefa39efp-1 / 256);
                 a.logprobs[r] = (float)(x - log((double)whole * 0x1p-47));
             }
         }
     }
+};
+
+template <class T, int NT, int WAVES>
+__global__ __launch_bounds__(NT, WAVES) void draw_kernel(Draw a, int64_t first) {
+    using D = Drawer<T, NT>;
+    __shared__ typename D::Shared sh;
+    if (threadIdx.x < 256) sh.power[threadIdx.x] = exp2((double)threadIdx.x / 256);
+    const int64_t r = first + blockIdx.x;
+    D{sh, row_of<T>(a.logits, r, a.inner), a.cols, 0.0f, 0.0f, 0.0, 0, false, 0.0}.draw(a, r);
 }
 
 // ---- log-probabilities --------------------------------------------------------------------------------------------------
@@ -843,13 +1084,15 @@ static int64_t adjust_runs(int64_t rows, int cols) {
     return (rows + run - 1) / run;
 }
 
+// One row a workgroup, without a loop over rows in the kernel: what such a loop keeps in registers for the next row costs it
+// half its waves.
 template <class T>
 static void draw_launch(const Draw &a, hipStream_t stream) {
-    const dim3 grid(grid_of(a.rows));
-    if (a.cols <= 2048) draw_kernel<T, 256, 8><<<grid, 256, 0, stream>>>(a);
-    else if (a.cols <= 8192) draw_kernel<T, 512, 16><<<grid, 512, 0, stream>>>(a);
-    else if (a.cols <= 32768) draw_kernel<T, 1024, 32><<<grid, 1024, 0, stream>>>(a);
-    else draw_kernel<T, 1024, 64><<<grid, 1024, 0, stream>>>(a);
+    for (int64_t first = 0; first < a.rows; first += 1 << 21) {
+        const unsigned grid = (unsigned)(a.rows - first < (1 << 21) ? a.rows - first : 1 << 21);
+        if (a.cols <= 1024) draw_kernel<T, 256, 8><<<grid, 256, 0, stream>>>(a, first);
+        else draw_kernel<T, 1024, 8><<<grid, 1024, 0, stream>>>(a, first);
+    }
 }
 
 static zbpe_status logprobs_of(const char *what, const zbpe_logprobs *p, Logprobs *out) {
