@@ -285,6 +285,12 @@ typedef struct zbpe_rows {
 zbpe_status zbpe_vocab_bytes(const uint16_t *triples, size_t n_merges, size_t vocab_size, uint32_t *offsets, uint8_t *bytes,
                              size_t cap, size_t *n_bytes);
 
+/* Host only. The tokens' bytes in the order in which grammar masks read them (32 bytes a token; opaque): writes
+ * zbpe_vocab_index_size(vocab_size) bytes (0 for a size outside 1 .. ZBPE_MAX_VOCAB). offsets and bytes as zbpe_vocab_bytes
+ * writes them. `index` is 16-byte aligned, on the host and where it is copied to. */
+size_t zbpe_vocab_index_size(size_t vocab_size);
+zbpe_status zbpe_vocab_index(const uint32_t *offsets, const uint8_t *bytes, size_t vocab_size, void *index);
+
 /* A grammar over a vocabulary, on the device: an automaton over bytes, and the tokens' bytes (zbpe_vocab_bytes). */
 typedef struct zbpe_grammar {
     const uint32_t *offsets;  /* [vocab_size + 1] */
@@ -294,6 +300,7 @@ typedef struct zbpe_grammar {
     const int32_t *next;      /* [n_states][256]: the state after a byte; any value outside 0 .. n_states - 1: refused */
     const uint8_t *accepting; /* [n_states], or NULL: no state accepts */
     int32_t n_states;
+    const void *index;        /* zbpe_vocab_index's, 16-byte aligned; zbpe_grammar_advance does not need it */
 } zbpe_grammar;
 
 /* Which tokens the grammar allows: row r of `masks` (words = (vocab_size + 31) / 32 u32) gets bit v % 32 of word v / 32 set

@@ -179,6 +179,59 @@ def test_token_bytes_refusals(merges, size, error, words):
         zbpe.token_bytes(merges, size)
 
 
+@pytest.mark.parametrize("size, skip", [(256, 0.0), (257, 1.0), (700, 0.2), (8192, 0.0), (8255, 0.1), (20000, 0.5)])
+def test_vocab_index(size, skip):
+    """every token once in its slice, in the order of its bytes; nothing written past the end"""
+    rng = np.random.default_rng(size)
+    merges = some_merges(size, rng, np.arange(256), most=30, skip=skip)
+    offsets, data = zbpe.token_bytes(np.array(merges).reshape(-1, 3), size)
+    L = zbpe.load_library()
+    n = (size + 63) // 64 * 64
+    assert L.zbpe_vocab_index_size(size) == n * 32 + n // 32
+    index = np.full(n * 32 + n // 32 + 64, 0xAA, np.uint8)
+    assert L.zbpe_vocab_index(offsets.ctypes.data, data.ctypes.data, size, index.ctypes.data) == 0
+    assert (index[-64:] == 0xAA).all()
+    heads, tails = index[:n * 16].reshape(n, 16), index[n * 16:n * 32].reshape(n, 16)
+    bounds = index[n * 32:n * 32 + n // 32].reshape(-1, 2)
+    classes = heads[:, :8].copy().view(np.uint64)[:, 0]
+    of_byte = {}
+    for base in range(0, size, 8192):
+        ids = [v for v in range(base, min(base + 8192, size)) if offsets[v] < offsets[v + 1]]
+        got = []
+        for e in range(base, base + len(ids)):
+            v, length = int(heads[e, 8]) + 256 * int(heads[e, 9]) + base, int(heads[e, 10])
+            b = data[offsets[v]:offsets[v + 1]].tobytes()
+            got.append((v, b[:8]))
+            assert length == min(len(b), 22)
+            assert heads[e, 11:].tobytes() + tails[e].tobytes() == b[:21].ljust(21, b"\0")
+            if len(b) == 1:
+                of_byte[b[0]] = int(classes[e])
+            want = 0
+            for c in b:
+                want |= of_byte[c] if c in of_byte else 0
+            if base or len(of_byte) == 256:
+                assert int(classes[e]) == want
+        assert sorted(v for v, _ in got) == ids
+        keys = [b.ljust(8, b"\0") for _, b in got]
+        assert keys == sorted(keys)
+        end = min(base + 8192, n)
+        assert not heads[base + len(ids):end].any() and not tails[base + len(ids):end].any()
+        for at in range(base, end, 64):
+            first = [data[offsets[v]] for v, _ in got[at - base:at - base + 64]]
+            assert tuple(bounds[at // 64]) == ((min(first), max(first)) if first else (255, 0))
+    assert all(bin(c).count("1") == 1 for c in of_byte.values())
+
+
+def test_vocab_index_refusals():
+    L = zbpe.load_library()
+    offsets, data, index = np.array([0, 2, 1], np.uint32), np.zeros(4, np.uint8), np.zeros(4096, np.uint8)
+    for size, words in ((2, "offsets of token 1 fall"), (0, "vocabulary of 0"), (65537, "vocabulary of 65537")):
+        assert L.zbpe_vocab_index(offsets.ctypes.data, data.ctypes.data, size, index.ctypes.data) == 5
+        assert words in L.zbpe_last_error(None).decode()
+    assert L.zbpe_vocab_index(offsets.ctypes.data, data.ctypes.data, 2, None) == 5
+    assert L.zbpe_vocab_index_size(0) == 0 and L.zbpe_vocab_index_size(65537) == 0
+
+
 def test_operators_refuse_tensors_off_the_gpu():
     z = torch.zeros(2, 300)
     for call in (lambda: zbpe.adjust_logits(z), lambda: zbpe.draw_tokens(z, torch.zeros(2)),
@@ -242,8 +295,8 @@ def test_c_entries_refuse_before_any_device_work():
     refused(L.zbpe_token_logprobs(0, None, logprobs(out=0)), "no logprobs")
     refused(L.zbpe_token_logprobs_grad(0, None, logprobs(), 4096, None), "type of the logits")
 
-    def masks(vocab=300, end=-1, states=5, rows=5, next=4096, out=4096):
-        return L.zbpe_grammar_masks(0, None, ops._GRAMMAR.pack(4096, 4096, vocab, end, next, 0, states), None, rows, out)
+    def masks(vocab=300, end=-1, states=5, rows=5, next=4096, out=4096, index=4096):
+        return L.zbpe_grammar_masks(0, None, ops._GRAMMAR.pack(4096, 4096, vocab, end, next, 0, states, index), None, rows, out)
 
     refused(masks(vocab=0), "vocabulary of 0")
     refused(masks(end=300), "end token")
@@ -251,6 +304,7 @@ def test_c_entries_refuse_before_any_device_work():
     refused(masks(rows=-1), "rows")
     refused(masks(next=0), "missing")
     refused(masks(out=0), "no masks")
+    refused(masks(index=0), "no index")
     assert L.zbpe_adjust_workspace(0, 300) == 0 and L.zbpe_adjust_workspace(-1, 300) == 0
 
 

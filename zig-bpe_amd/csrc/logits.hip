@@ -121,6 +121,7 @@ struct Automaton {
     const uint8_t *bytes;
     const int32_t *next;
     const uint8_t *accepting;
+    const void *index;
     int vocab, end, n;
 };
 
@@ -132,23 +133,168 @@ __device__ __forceinline__ int walk(const Automaton &g, int s, uint32_t at, uint
     return inside(g, s) ? s : -1;
 }
 
-__global__ __launch_bounds__(256) void grammar_masks_kernel(Automaton g, const int32_t *states, int64_t rows, uint32_t *masks, int slices) {
-    const int words = (g.vocab + 31) / 32, lane = threadIdx.x & 63;
-    for (int64_t w = blockIdx.x; w < rows * slices; w += gridDim.x) {
-        const int64_t r = w / slices;
-        const int v = (int)(w % slices) * 256 + (int)threadIdx.x;
-        const int s = states ? states[r] : (int)r;
-        bool on = false;
-        if (v < g.vocab && inside(g, s)) {
-            if (v == g.end) on = g.accepting && g.accepting[s];
-            else {
-                const uint32_t a = g.offsets[v], b = g.offsets[v + 1];
-                on = a < b && walk(g, s, a, b) >= 0;
+// One workgroup makes one state's bits of one slice of ids after another. Most tokens need no walk:
+//   - The slice's tokens come in the order of their bytes (vocab.hpp), so 64 neighbours begin alike; where the state refuses all
+//     of a wave's first bytes, its tokens are not even read.
+//   - Most bytes of an answer leave the state as it is (the inside of a string, a number's digits). A token carries the set of its
+//     bytes' classes; when no class in it holds a byte that changes the state, the token is allowed.
+//   - Of the others most end at their second byte.
+// What is left is queued and walked by full waves. The rows of the automaton that such walks need most, the state's own and up
+// to seven that follow it, are in shared memory, their entries replaced by the places of these rows (0 .. ROWS - 1; other states
+// follow, -1: refused). The bits return to the order of ids in shared memory.
+template <int NT>
+__global__ __launch_bounds__(NT) void grammar_masks_kernel(Automaton g, const int32_t *states, int64_t rows, uint32_t *masks, int slices, int per) {
+    constexpr int GROUPS = INDEX_SLICE / 64, ROWS = 8;
+    __shared__ int next[ROWS][256];
+    __shared__ int place[ROWS];  // the states of these rows
+    __shared__ uint32_t live[8], turns[2];  // the bytes that the state takes; the classes with a byte that changes it
+    __shared__ uint32_t bits[INDEX_SLICE / 32];
+    __shared__ uint16_t queue[INDEX_SLICE];
+    __shared__ uint8_t list[GROUPS];
+    __shared__ int listed, queued;
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, words = (g.vocab + 31) / 32;
+    const int parts = (slices + per - 1) / per;
+    const IndexView index(g.index, g.vocab);
+    for (int64_t w = blockIdx.x; w < rows * parts; w += gridDim.x) {
+        const int64_t r = w / parts;
+        const int first_slice = (int)(w % parts) * per, last_slice = first_slice + per < slices ? first_slice + per : slices;
+        const int s0 = states ? states[r] : (int)r;
+        const bool known = inside(g, s0);
+        __syncthreads();
+        if (t < 2) turns[t] = 0;
+        __syncthreads();
+        if (t < 256) {
+            const int to = known ? g.next[(int64_t)s0 * 256 + t] : -1;
+            const bool on = inside(g, to);
+            next[0][t] = on ? to : -1;
+            const uint64_t b = __ballot(on);
+            if (lane == 0) live[t >> 5] = (uint32_t)b;
+            if (lane == 32) live[t >> 5] = (uint32_t)(b >> 32);
+            const int c = byte_class(t);
+            uint32_t low = to != s0 && c < 32 ? 1u << c : 0u, high = to != s0 && c >= 32 ? 1u << (c - 32) : 0u;
+            for (int d = 32; d; d >>= 1) {
+                low |= __shfl_xor(low, d);
+                high |= __shfl_xor(high, d);
+            }
+            if (lane == 0) {
+                atomicOr(&turns[0], low);
+                atomicOr(&turns[1], high);
             }
         }
-        const uint64_t bits = __ballot(on);
-        const int word = (v - lane) / 32 + (lane >> 5);
-        if ((lane & 31) == 0 && word < words) masks[r * words + word] = (uint32_t)(bits >> (lane & 32));
+        __syncthreads();
+        if (wave == 0) {  // the first states that follow, each once
+            int to[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) to[i] = next[0][i * 64 + lane];
+            int chosen = s0;
+            for (int k = 0; k < ROWS; k++) {
+                int mine = -1;
+#pragma unroll
+                for (int i = 3; i >= 0; i--) {
+                    if (to[i] == chosen) to[i] = -1;
+                    if (to[i] >= 0) mine = to[i];
+                }
+                if (lane == 0) place[k] = chosen;
+                const uint64_t b = __ballot(mine >= 0);
+                chosen = b ? __shfl(mine, __ffsll((unsigned long long)b) - 1) : -1;
+            }
+        }
+        __syncthreads();
+        for (int i = t; i < ROWS * 256; i += NT) {
+            const int s = place[i >> 8];
+            int to = i < 256 ? next[0][i] : s >= 0 && known ? g.next[(int64_t)s * 256 + (i & 255)] : -1;
+            if (!inside(g, to)) to = -1;
+            else {
+                int at = to + ROWS;
+#pragma unroll
+                for (int k = ROWS - 1; k >= 0; k--)
+                    if (to == place[k]) at = k;
+                to = at;
+            }
+            next[i >> 8][i & 255] = to;
+        }
+        const uint32_t turns_low = turns[0], turns_high = turns[1];
+        for (int slice = first_slice; slice < last_slice; slice++) {
+            const int base = slice * INDEX_SLICE;
+            const int groups = min(GROUPS, (g.vocab - base + 63) / 64);
+            for (int i = t; i < INDEX_SLICE / 32; i += NT) {
+                const bool ends = g.end >= 0 && g.end / 32 == base / 32 + i && known && g.accepting && g.accepting[s0];
+                bits[i] = ends ? 1u << (g.end & 31) : 0u;
+            }
+            if (t == 0) listed = queued = 0;
+            __syncthreads();
+            if (t < groups) {
+                const IndexBounds x = index.bounds[base / 64 + t];
+                uint32_t any = 0;
+                for (int i = x.lo >> 5; i <= x.hi >> 5; i++) {
+                    uint32_t m = live[i];
+                    if (i == x.lo >> 5) m &= ~0u << (x.lo & 31);
+                    if (i == x.hi >> 5) m &= ~0u >> (31 - (x.hi & 31));
+                    any |= m;
+                }
+                if (any) list[atomicAdd(&listed, 1)] = (uint8_t)t;  // (in any order: each group has bits of its own)
+            }
+            __syncthreads();
+            const int n = listed;
+            for (int i = wave; i < n; i += NT / 64) {
+                const int at = list[i] * 64 + lane;
+                const IndexHead x = index.heads[base + at];
+                const int id = x.id(), length = x.length();
+                bool on = false, open = false;
+                if (length && base + id != g.end) {
+                    on = !((x.classes[0] & turns_low) | (x.classes[1] & turns_high));
+                    if (!on) {
+                        const int s = next[0][x.byte(0)];
+                        if (s >= 0) {
+                            if (length == 1) on = true;
+                            else if (s >= ROWS) open = true;
+                            else if (next[s][x.byte(1)] >= 0) {
+                                on = length == 2;
+                                open = !on;
+                            }
+                        }
+                    }
+                }
+                if (on) atomicOr(&bits[id >> 5], 1u << (id & 31));
+                const uint64_t b = __ballot(open);
+                if (b) {
+                    int from = 0;
+                    if (lane == 0) from = atomicAdd(&queued, __popcll(b));
+                    from = __shfl(from, 0);
+                    if (open) queue[from + __popcll(b & ((1ull << lane) - 1))] = (uint16_t)at;
+                }
+            }
+            __syncthreads();
+            const int m = queued;
+            for (int i = t; i < m; i += NT) {
+                const int at = queue[i];
+                const IndexHead x = index.heads[base + at];
+                const IndexTail y = index.tails[base + at];
+                const int id = x.id(), length = x.length();
+                int s = 0;
+#pragma unroll
+                for (int j = 0; j < INDEX_BYTES; j++) {
+                    const bool on = s >= 0 && j < length;
+                    if (!__any(on)) break;
+                    const int b = j < INDEX_HEAD ? x.byte(j) : y.byte(j - INDEX_HEAD);
+                    if (on) {
+                        if (s < ROWS) s = next[s][b];
+                        else {
+                            s = g.next[(int64_t)(s - ROWS) * 256 + b];
+                            s = inside(g, s) ? s == s0 ? 0 : s + ROWS : -1;
+                        }
+                    }
+                }
+                if (length > INDEX_BYTES && s >= 0) {
+                    const uint32_t from = g.offsets[base + id] + INDEX_BYTES, to = g.offsets[base + id + 1];
+                    s = walk(g, s < ROWS ? place[s] : s - ROWS, from, to);
+                }
+                if (s >= 0) atomicOr(&bits[id >> 5], 1u << (id & 31));
+            }
+            __syncthreads();
+            for (int i = t; i < INDEX_SLICE / 32 && base / 32 + i < words; i += NT) masks[r * words + base / 32 + i] = bits[i];
+            __syncthreads();
+        }
     }
 }
 
@@ -1024,7 +1170,7 @@ static zbpe_status grammar_of(const char *what, const zbpe_grammar *g, int64_t r
     if (g->n_states < 0 || g->n_states >= (1 << 23)) return refuse(ZBPE_INVALID_ARGUMENT, "%s: %d states (fewer than 2^23)", what, g->n_states);
     if (rows < 0 || rows >= (1ll << 40)) return refuse(ZBPE_INVALID_ARGUMENT, "%s: %lld rows", what, (long long)rows);
     if (!g->offsets || !g->bytes || (!g->next && g->n_states)) return refuse(ZBPE_INVALID_ARGUMENT, "%s: an array of the grammar is missing", what);
-    *out = Automaton{g->offsets, g->bytes, g->next, g->accepting, g->vocab_size, g->end_token, g->n_states};
+    *out = Automaton{g->offsets, g->bytes, g->next, g->accepting, g->index, g->vocab_size, g->end_token, g->n_states};
     return ZBPE_OK;
 }
 
@@ -1137,6 +1283,22 @@ zbpe_status zbpe_vocab_bytes(const uint16_t *triples, size_t n_merges, size_t vo
     }
 }
 
+size_t zbpe_vocab_index_size(size_t vocab_size) { return vocab_size < 1 || vocab_size > ZBPE_MAX_VOCAB ? 0 : index_size(vocab_size); }
+
+zbpe_status zbpe_vocab_index(const uint32_t *offsets, const uint8_t *bytes, size_t vocab_size, void *index) {
+    if (!offsets || !bytes || !index) return refuse(ZBPE_INVALID_ARGUMENT, "zbpe_vocab_index: an array is missing");
+    if (vocab_size < 1 || vocab_size > ZBPE_MAX_VOCAB)
+        return refuse(ZBPE_INVALID_ARGUMENT, "zbpe_vocab_index: a vocabulary of %zu (1 to %d)", vocab_size, ZBPE_MAX_VOCAB);
+    for (size_t v = 0; v < vocab_size; v++)
+        if (offsets[v] > offsets[v + 1]) return refuse(ZBPE_INVALID_ARGUMENT, "zbpe_vocab_index: the offsets of token %zu fall", v);
+    try {
+        index_tokens(offsets, bytes, vocab_size, index);
+        return ZBPE_OK;
+    } catch (const std::bad_alloc &) {
+        return refuse(ZBPE_OUT_OF_MEMORY, "zbpe_vocab_index: out of host memory");
+    }
+}
+
 zbpe_status zbpe_grammar_masks(int device, void *stream, const zbpe_grammar *grammar, const int32_t *states, int64_t rows,
                                uint32_t *masks) {
     const char *what = "zbpe_grammar_masks";
@@ -1144,10 +1306,16 @@ zbpe_status zbpe_grammar_masks(int device, void *stream, const zbpe_grammar *gra
     zbpe_status s = grammar_of(what, grammar, rows, &g);
     if (s != ZBPE_OK || !rows) return s;
     if (!masks) return refuse(ZBPE_INVALID_ARGUMENT, "%s: no masks", what);
+    if (!g.index) return refuse(ZBPE_INVALID_ARGUMENT, "%s: no index of the tokens", what);
     OnDevice on;
     if ((s = on.go(device)) != ZBPE_OK) return s;
-    const int slices = (g.vocab + 255) / 256;
-    grammar_masks_kernel<<<grid_of(rows * slices), 256, 0, (hipStream_t)stream>>>(g, states, rows, masks, slices);
+    // a workgroup's slices share what it finds out about its state; few rows need many workgroups
+    const int slices = (g.vocab + INDEX_SLICE - 1) / INDEX_SLICE;
+    const int64_t fit = rows * slices / 4096;
+    const int per = (int)(fit < 1 ? 1 : fit < slices ? fit : slices);
+    const int64_t parts = rows * ((slices + per - 1) / per);
+    if (parts < 512) grammar_masks_kernel<1024><<<grid_of(parts), 1024, 0, (hipStream_t)stream>>>(g, states, rows, masks, slices, per);
+    else grammar_masks_kernel<512><<<grid_of(parts), 512, 0, (hipStream_t)stream>>>(g, states, rows, masks, slices, per);
     return launched(what);
 }
 

@@ -153,7 +153,7 @@ EXPORTS = (
     "zbpe_train", "zbpe_upload", "zbpe_train_resident", "zbpe_encode", "zbpe_verify_counts", "zbpe_tokens",
     "zbpe_set_option", "zbpe_format_time_stats", "zbpe_bench_scan", "zbpe_bench_train_scan", "zbpe_merge_log", "zbpe_trace", "zbpe_scan_log", "zbpe_compaction_log", "zbpe_halt_log", "zbpe_zig_order_winner", "zbpe_version",
     "zbpe_stats_size", "zbpe_bench_recount",
-    "zbpe_vocab_bytes", "zbpe_grammar_masks", "zbpe_grammar_advance", "zbpe_adjust_logits", "zbpe_adjust_workspace",
+    "zbpe_vocab_bytes", "zbpe_vocab_index_size", "zbpe_vocab_index", "zbpe_grammar_masks", "zbpe_grammar_advance", "zbpe_adjust_logits", "zbpe_adjust_workspace",
     "zbpe_adjust_logits_grad", "zbpe_draw_tokens", "zbpe_token_logprobs", "zbpe_token_logprobs_grad", "zbpe_struct_size",
 )
 MERGE_LOG_COLUMNS = ("key", "count", "live", "ties", "list_scan", "list_len", "key_live", "range")
@@ -239,6 +239,8 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
     if hasattr(L, "zbpe_draw_tokens"):  # (structures go as packed bytes: zbpe/logits.py)
         i, i64 = ctypes.c_int, ctypes.c_int64
         L.zbpe_vocab_bytes.argtypes = [vp, sz, sz, vp, vp, sz, ctypes.POINTER(sz)]
+        L.zbpe_vocab_index_size.argtypes = [sz]
+        L.zbpe_vocab_index.argtypes = [vp, vp, sz, vp]
         L.zbpe_grammar_masks.argtypes = [i, vp, vp, vp, i64, vp]
         L.zbpe_grammar_advance.argtypes = [i, vp, vp, vp, vp, i64, vp]
         L.zbpe_adjust_logits.argtypes = [i, vp, vp]
@@ -250,7 +252,7 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
         L.zbpe_struct_size.argtypes = [i]
     for name in EXPORTS:
         if name not in ("zbpe_destroy", "zbpe_last_error", "zbpe_version", "zbpe_stats_size") and hasattr(L, name):
-            getattr(L, name).restype = ctypes.c_size_t if name in ("zbpe_adjust_workspace", "zbpe_struct_size") else ctypes.c_int
+            getattr(L, name).restype = ctypes.c_size_t if name in ("zbpe_adjust_workspace", "zbpe_struct_size", "zbpe_vocab_index_size") else ctypes.c_int
     if hasattr(L, "zbpe_stats_size"):  # the caller-allocated zbpe_stats must match the library's layout
         L.zbpe_stats_size.restype = ctypes.c_size_t
         if L.zbpe_stats_size() != ctypes.sizeof(Stats):

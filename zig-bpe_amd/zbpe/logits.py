@@ -28,7 +28,7 @@ _INTS = {torch.int32: 3, torch.int64: 4}
 
 # include/zbpe.h's structures, field by field ("@": native alignment, as a C compiler lays them out)
 _ROWS = "Pqqi0q"
-_GRAMMAR = struct.Struct("@PPiiPPi0q")
+_GRAMMAR = struct.Struct("@PPiiPPiP")
 _ADJUST = struct.Struct("@Iiqq" + 3 * _ROWS + "qPPPPPPPPiiPqP")
 _DRAW = struct.Struct("@Iiqq" + _ROWS + "PPPPPPP")
 _LOGPROBS = struct.Struct("@Iiqq" + _ROWS + "PiPPP")
@@ -176,6 +176,10 @@ class Vocabulary:
             self.device = torch.device("cuda", torch.cuda.current_device())
         self.offsets = torch.from_numpy(offsets.view(np.int32)).to(self.device)
         self.bytes = torch.from_numpy(data).to(self.device)
+        L = _library()
+        index = np.empty(L.zbpe_vocab_index_size(self.size), np.uint8)
+        _check(L.zbpe_vocab_index(_ptr(offsets), _ptr(data), self.size, _ptr(index)))
+        self.index = torch.from_numpy(index).to(self.device)
 
     def lengths(self) -> torch.Tensor:
         """Bytes of each token, int32 [size]; 0 where it has none."""
@@ -221,7 +225,7 @@ class Grammar:
     def _packed(self) -> bytes:
         v = self.vocabulary
         return _GRAMMAR.pack(v.offsets.data_ptr(), v.bytes.data_ptr(), v.size, v.end_token, self.next.data_ptr(),
-                             0 if self.accepting is None else self.accepting.data_ptr(), self.states)
+                             0 if self.accepting is None else self.accepting.data_ptr(), self.states, v.index.data_ptr())
 
     def _vector(self, x: torch.Tensor, name: str) -> torch.Tensor:
         _is_tensor(x, name)
