@@ -11,6 +11,7 @@
 #include "../../include/zbpe.h"
 #include "logits.hpp"
 #include "vocab.hpp"
+#include "wave.hpp"
 
 namespace zbpe {
 
@@ -133,35 +134,36 @@ __device__ __forceinline__ int walk(const Automaton &g, int s, uint32_t at, uint
     return inside(g, s) ? s : -1;
 }
 
-// One workgroup makes one state's bits of one slice of ids after another. Most tokens need no walk:
-//   - The slice's tokens come in the order of their bytes (vocab.hpp), so 64 neighbours begin alike; where the state refuses all
-//     of a wave's first bytes, its tokens are not even read.
+// One workgroup makes one state's bits of some slices of ids. Most tokens need no walk:
+//   - A slice's tokens come in the order of their bytes (vocab.hpp), so 64 neighbours begin alike; where the state refuses all of
+//     their first bytes, they are not even read.
 //   - Most bytes of an answer leave the state as it is (the inside of a string, a number's digits). A token carries the set of its
 //     bytes' classes; when no class in it holds a byte that changes the state, the token is allowed.
 //   - Of the others most end at their second byte.
-// What is left is queued and walked by full waves. The rows of the automaton that such walks need most, the state's own and up
-// to seven that follow it, are in shared memory, their entries replaced by the places of these rows (0 .. ROWS - 1; other states
-// follow, -1: refused). The bits return to the order of ids in shared memory.
+// Each wave queues what is left and walks it 64 at a time. The rows of the automaton that such walks need most, the state's own
+// and up to seven that follow it, are in shared memory, their entries replaced by the places of these rows (0 .. ROWS - 1; other
+// states follow, -1: refused). The bits return to the order of ids in shared memory.
 template <int NT>
 __global__ __launch_bounds__(NT) void grammar_masks_kernel(Automaton g, const int32_t *states, int64_t rows, uint32_t *masks, int slices, int per) {
-    constexpr int GROUPS = INDEX_SLICE / 64, ROWS = 8;
+    constexpr int ROWS = 8, SLICES = ZBPE_MAX_VOCAB / INDEX_SLICE, SLICE_WORDS = INDEX_SLICE / 32;
     __shared__ int next[ROWS][256];
     __shared__ int place[ROWS];  // the states of these rows
-    __shared__ uint32_t live[8], turns[2];  // the bytes that the state takes; the classes with a byte that changes it
-    __shared__ uint32_t bits[INDEX_SLICE / 32];
-    __shared__ uint16_t queue[INDEX_SLICE];
-    __shared__ uint8_t list[GROUPS];
-    __shared__ int listed, queued;
+    __shared__ uint32_t live[8], turns[2][4];  // the bytes that the state takes; the classes with a byte that changes it
+    __shared__ uint32_t bits[SLICES * SLICE_WORDS];
+    __shared__ uint16_t list[SLICES * INDEX_SLICE / 64];
+    __shared__ uint16_t queues[NT / 64][128];
+    __shared__ int listed;
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, words = (g.vocab + 31) / 32;
     const int parts = (slices + per - 1) / per;
     const IndexView index(g.index, g.vocab);
+    uint16_t *queue = queues[wave];
     for (int64_t w = blockIdx.x; w < rows * parts; w += gridDim.x) {
         const int64_t r = w / parts;
         const int first_slice = (int)(w % parts) * per, last_slice = first_slice + per < slices ? first_slice + per : slices;
+        const int first_word = first_slice * SLICE_WORDS, last_word = min(last_slice * SLICE_WORDS, words);
+        const int first_group = first_slice * (INDEX_SLICE / 64), last_group = min(last_slice * (INDEX_SLICE / 64), (g.vocab + 63) / 64);
         const int s0 = states ? states[r] : (int)r;
         const bool known = inside(g, s0);
-        __syncthreads();
-        if (t < 2) turns[t] = 0;
         __syncthreads();
         if (t < 256) {
             const int to = known ? g.next[(int64_t)s0 * 256 + t] : -1;
@@ -171,18 +173,30 @@ __global__ __launch_bounds__(NT) void grammar_masks_kernel(Automaton g, const in
             if (lane == 0) live[t >> 5] = (uint32_t)b;
             if (lane == 32) live[t >> 5] = (uint32_t)(b >> 32);
             const int c = byte_class(t);
-            uint32_t low = to != s0 && c < 32 ? 1u << c : 0u, high = to != s0 && c >= 32 ? 1u << (c - 32) : 0u;
-            for (int d = 32; d; d >>= 1) {
-                low |= __shfl_xor(low, d);
-                high |= __shfl_xor(high, d);
-            }
+            const uint32_t low = wave_or_u32(to != s0 && c < 32 ? 1u << c : 0u), high = wave_or_u32(to != s0 && c >= 32 ? 1u << (c - 32) : 0u);
             if (lane == 0) {
-                atomicOr(&turns[0], low);
-                atomicOr(&turns[1], high);
+                turns[0][wave] = low;
+                turns[1][wave] = high;
             }
         }
+        for (int i = t; i < last_word - first_word; i += NT) {
+            const bool ends = g.end >= 0 && g.end / 32 == first_word + i && known && g.accepting && g.accepting[s0];
+            bits[i] = ends ? 1u << (g.end & 31) : 0u;
+        }
+        if (t == 0) listed = 0;
         __syncthreads();
-        if (wave == 0) {  // the first states that follow, each once
+        for (int i = first_group + t; i < last_group; i += NT) {
+            const IndexBounds x = index.bounds[i];
+            uint32_t any = 0;
+            for (int i = x.lo >> 5; i <= x.hi >> 5; i++) {
+                uint32_t m = live[i];
+                if (i == x.lo >> 5) m &= ~0u << (x.lo & 31);
+                if (i == x.hi >> 5) m &= ~0u >> (31 - (x.hi & 31));
+                any |= m;
+            }
+            if (any) list[atomicAdd(&listed, 1)] = (uint16_t)i;  // (in any order: each group has bits of its own)
+        }
+        if (wave == NT / 64 - 1) {  // the first states that follow, each once
             int to[4];
 #pragma unroll
             for (int i = 0; i < 4; i++) to[i] = next[0][i * 64 + lane];
@@ -196,7 +210,7 @@ __global__ __launch_bounds__(NT) void grammar_masks_kernel(Automaton g, const in
                 }
                 if (lane == 0) place[k] = chosen;
                 const uint64_t b = __ballot(mine >= 0);
-                chosen = b ? __shfl(mine, __ffsll((unsigned long long)b) - 1) : -1;
+                chosen = b ? (int)lane_bcast((uint32_t)mine, __ffsll((unsigned long long)b) - 1) : -1;
             }
         }
         __syncthreads();
@@ -213,88 +227,73 @@ __global__ __launch_bounds__(NT) void grammar_masks_kernel(Automaton g, const in
             }
             next[i >> 8][i & 255] = to;
         }
-        const uint32_t turns_low = turns[0], turns_high = turns[1];
-        for (int slice = first_slice; slice < last_slice; slice++) {
-            const int base = slice * INDEX_SLICE;
-            const int groups = min(GROUPS, (g.vocab - base + 63) / 64);
-            for (int i = t; i < INDEX_SLICE / 32; i += NT) {
-                const bool ends = g.end >= 0 && g.end / 32 == base / 32 + i && known && g.accepting && g.accepting[s0];
-                bits[i] = ends ? 1u << (g.end & 31) : 0u;
-            }
-            if (t == 0) listed = queued = 0;
-            __syncthreads();
-            if (t < groups) {
-                const IndexBounds x = index.bounds[base / 64 + t];
-                uint32_t any = 0;
-                for (int i = x.lo >> 5; i <= x.hi >> 5; i++) {
-                    uint32_t m = live[i];
-                    if (i == x.lo >> 5) m &= ~0u << (x.lo & 31);
-                    if (i == x.hi >> 5) m &= ~0u >> (31 - (x.hi & 31));
-                    any |= m;
-                }
-                if (any) list[atomicAdd(&listed, 1)] = (uint8_t)t;  // (in any order: each group has bits of its own)
-            }
-            __syncthreads();
-            const int n = listed;
-            for (int i = wave; i < n; i += NT / 64) {
-                const int at = list[i] * 64 + lane;
-                const IndexHead x = index.heads[base + at];
-                const int id = x.id(), length = x.length();
-                bool on = false, open = false;
-                if (length && base + id != g.end) {
-                    on = !((x.classes[0] & turns_low) | (x.classes[1] & turns_high));
-                    if (!on) {
-                        const int s = next[0][x.byte(0)];
-                        if (s >= 0) {
-                            if (length == 1) on = true;
-                            else if (s >= ROWS) open = true;
-                            else if (next[s][x.byte(1)] >= 0) {
-                                on = length == 2;
-                                open = !on;
-                            }
-                        }
-                    }
-                }
-                if (on) atomicOr(&bits[id >> 5], 1u << (id & 31));
-                const uint64_t b = __ballot(open);
-                if (b) {
-                    int from = 0;
-                    if (lane == 0) from = atomicAdd(&queued, __popcll(b));
-                    from = __shfl(from, 0);
-                    if (open) queue[from + __popcll(b & ((1ull << lane) - 1))] = (uint16_t)at;
-                }
-            }
-            __syncthreads();
-            const int m = queued;
-            for (int i = t; i < m; i += NT) {
-                const int at = queue[i];
-                const IndexHead x = index.heads[base + at];
-                const IndexTail y = index.tails[base + at];
-                const int id = x.id(), length = x.length();
-                int s = 0;
+        __syncthreads();
+        const uint32_t turns_low = turns[0][0] | turns[0][1] | turns[0][2] | turns[0][3];
+        const uint32_t turns_high = turns[1][0] | turns[1][1] | turns[1][2] | turns[1][3];
+
+        auto allow = [&](int id) { atomicOr(&bits[(id >> 5) - first_word], 1u << (id & 31)); };
+        auto walk_queued = [&](int i) {
+            const int at = queue[i];
+            const IndexHead x = index.heads[at];
+            const IndexTail y = index.tails[at];
+            const int id = at / INDEX_SLICE * INDEX_SLICE + x.id(), length = x.length();
+            int s = 0;
 #pragma unroll
-                for (int j = 0; j < INDEX_BYTES; j++) {
-                    const bool on = s >= 0 && j < length;
-                    if (!__any(on)) break;
-                    const int b = j < INDEX_HEAD ? x.byte(j) : y.byte(j - INDEX_HEAD);
-                    if (on) {
-                        if (s < ROWS) s = next[s][b];
-                        else {
-                            s = g.next[(int64_t)(s - ROWS) * 256 + b];
-                            s = inside(g, s) ? s == s0 ? 0 : s + ROWS : -1;
+            for (int j = 0; j < INDEX_BYTES; j++) {
+                const bool on = s >= 0 && j < length;
+                if (!__any(on)) break;
+                const int b = j < INDEX_HEAD ? x.byte(j) : y.byte(j - INDEX_HEAD);
+                if (on) {
+                    if (s < ROWS) s = next[s][b];
+                    else {
+                        s = g.next[(int64_t)(s - ROWS) * 256 + b];
+                        s = inside(g, s) ? s == s0 ? 0 : s + ROWS : -1;
+                    }
+                }
+            }
+            if (length > INDEX_BYTES && s >= 0) s = walk(g, s < ROWS ? place[s] : s - ROWS, g.offsets[id] + INDEX_BYTES, g.offsets[id + 1]);
+            if (s >= 0) allow(id);
+        };
+
+        const int n = listed;
+        int queued = 0, at = 0;
+        IndexHead ahead{};
+        if (wave < n) ahead = index.heads[at = list[wave] * 64 + lane];
+        for (int i = wave; i < n; i += NT / 64) {
+            const IndexHead x = ahead;
+            const int here = at;
+            if (i + NT / 64 < n) ahead = index.heads[at = list[i + NT / 64] * 64 + lane];
+            const int id = here / INDEX_SLICE * INDEX_SLICE + x.id(), length = x.length();
+            bool on = false, open = false;
+            if (length && id != g.end) {
+                on = !((x.classes[0] & turns_low) | (x.classes[1] & turns_high));
+                if (!on) {
+                    const int s = next[0][x.byte(0)];
+                    if (s >= 0) {
+                        if (length == 1) on = true;
+                        else if (s >= ROWS) open = true;
+                        else if (next[s][x.byte(1)] >= 0) {
+                            on = length == 2;
+                            open = !on;
                         }
                     }
                 }
-                if (length > INDEX_BYTES && s >= 0) {
-                    const uint32_t from = g.offsets[base + id] + INDEX_BYTES, to = g.offsets[base + id + 1];
-                    s = walk(g, s < ROWS ? place[s] : s - ROWS, from, to);
-                }
-                if (s >= 0) atomicOr(&bits[id >> 5], 1u << (id & 31));
             }
-            __syncthreads();
-            for (int i = t; i < INDEX_SLICE / 32 && base / 32 + i < words; i += NT) masks[r * words + base / 32 + i] = bits[i];
-            __syncthreads();
+            if (on) allow(id);
+            const uint64_t b = __ballot(open);
+            if (open) queue[queued + __popcll(b & ((1ull << lane) - 1))] = (uint16_t)here;
+            queued += __popcll(b);
+            if (queued >= 64) {
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                queued -= 64;
+                walk_queued(queued + lane);
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            }
         }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if (lane < queued) walk_queued(lane);
+        __syncthreads();
+        for (int i = t; i < last_word - first_word; i += NT) masks[r * words + first_word + i] = bits[i];
     }
 }
 

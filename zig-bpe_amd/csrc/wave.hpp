@@ -38,6 +38,14 @@ __device__ __attribute__((always_inline)) inline uint32_t wave_sum_u32(uint32_t 
     return (uint32_t)__builtin_amdgcn_readlane((int)x, 0) + (uint32_t)__builtin_amdgcn_readlane((int)x, 16) +
            (uint32_t)__builtin_amdgcn_readlane((int)x, 32) + (uint32_t)__builtin_amdgcn_readlane((int)x, 48);
 }
+__device__ __attribute__((always_inline)) inline uint32_t wave_or_u32(uint32_t x) {
+    x |= dpp_mov<0xB1>(x);
+    x |= dpp_mov<0x4E>(x);
+    x |= dpp_mov<0x141>(x);
+    x |= dpp_mov<0x140>(x);
+    return (uint32_t)__builtin_amdgcn_readlane((int)x, 0) | (uint32_t)__builtin_amdgcn_readlane((int)x, 16) |
+           (uint32_t)__builtin_amdgcn_readlane((int)x, 32) | (uint32_t)__builtin_amdgcn_readlane((int)x, 48);
+}
 // lane l's x, as a scalar
 __device__ __attribute__((always_inline)) inline uint32_t lane_bcast(uint32_t x, int l) {
     return (uint32_t)__builtin_amdgcn_readlane((int)x, l);
