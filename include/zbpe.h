@@ -349,7 +349,7 @@ zbpe_status zbpe_adjust_logits(int device, void *stream, const zbpe_adjust *args
 /* Its gradient: `args` as in the call, args->out the gradient of its output (only read), args->logits the same logits. Writes
  * grad_logits (the logits' type, rows of its own), grad_bias [cols] and grad_bias_values [rows][n_biases]; each may be NULL.
  * A masked element passes no gradient. grad_bias needs a workspace of zbpe_adjust_workspace(rows, cols) bytes, which no
- * other call uses until this one is done; it sums rows in an order that depends on rows and cols alone. */
+ * other call uses until this one is done; it sums rows in an order that depends on rows, cols and the type alone. */
 size_t zbpe_adjust_workspace(int64_t rows, int32_t cols);
 zbpe_status zbpe_adjust_logits_grad(int device, void *stream, const zbpe_adjust *args, const zbpe_rows *grad_logits,
                                     float *grad_bias, float *grad_bias_values, void *workspace, size_t workspace_size);

@@ -40,8 +40,28 @@ __device__ __forceinline__ T *row_of(const Rows &m, int64_t r, int64_t per) {
     return (T *)m.data + at;
 }
 
+// A row's place in both levels, for walks over consecutive rows: one division for all of them.
+struct RowAt {
+    int64_t outer, inner;
+    __device__ __forceinline__ RowAt(int64_t r, int64_t per) : outer(r / per), inner(r % per) {}
+    __device__ __forceinline__ void next(int64_t per) {
+        if (++inner == per) {
+            inner = 0;
+            outer++;
+        }
+    }
+    template <class T>
+    __device__ __forceinline__ T *of(const Rows &m) const { return (T *)m.data + outer * m.outer + inner * m.inner; }
+};
+
 using f16 = _Float16;
 using bf16 = __bf16;
+
+// The same number, worked with anew: what is computed from it for the ends of rows is not kept in registers through whole loops.
+__device__ __forceinline__ int afresh(int x) {
+    asm volatile("" : "+s"(x));
+    return x;
+}
 
 // 16 bytes of elements. Rows may start at any element (an odd number of columns): the copies below are 16-byte loads and
 // stores at the element's alignment, which global memory allows.
@@ -80,9 +100,10 @@ __device__ __forceinline__ void store_floats(T *row, int col, int cols, const fl
         for (int e = 0; e < N; e++) x[e] = (T)z[e];
         __builtin_memcpy(row + col, x, sizeof x);
     } else {
+        const int left = afresh(cols) - col;
 #pragma unroll
         for (int e = 0; e < N; e++)
-            if (col + e < cols) row[col + e] = (T)z[e];
+            if (e < left) row[col + e] = (T)z[e];
     }
 }
 
@@ -313,205 +334,386 @@ __global__ __launch_bounds__(256) void grammar_advance_kernel(Automaton g, const
 
 // ---- penalties, biases and masks ----------------------------------------------------------------------------------------
 
-constexpr int ADJUST_THREADS = 256, ADJUST_EACH = 16, ADJUST_SLICE = ADJUST_THREADS * ADJUST_EACH;
+// A workgroup takes a slice of columns over a run of rows, 32 bytes of logits a thread. What a row needs from memory is on its
+// way while the row before it is worked on. The row's history is counted in shared memory: a bit for each column that is in it
+// (the bits of one load's columns in one byte, which is 0 for most loads) and how often behind the prompt. Whoever uses a bit
+// or a count clears it.
+constexpr int ADJUST_THREADS = 512, ADJUST_PACKS = 2, ADJUST_RUN = 32;
+constexpr int ADJUST_GROUPS = 3;  // on a CU at a time: 6 waves on a SIMD leave 80 registers to a thread
+template <class T>
+constexpr int ADJUST_SLICE = ADJUST_THREADS * ADJUST_PACKS * Pack<T>::N;
 
 struct Adjust {
     Rows logits, out, history;
-    int64_t rows, inner, mask_rows;
-    int cols, slices, words, n_biases, wide_ids;
+    int64_t rows, inner, mask_rows, runs;
+    int cols, slices, run, words, n_biases, wide_ids;
     int64_t history_len;
     const int32_t *lengths, *prompt_lengths, *bias_tokens, *states;
     const float *repetition, *presence, *frequency, *bias, *bias_values;
     const uint32_t *masks;
 };
 
-// The row of masks of logits row r; null: everything is masked.
-__device__ __forceinline__ const uint32_t *mask_row(const Adjust &a, int64_t r) {
-    const int64_t m = a.states ? a.states[r] : a.mask_rows == 1 ? 0 : r;
-    return m >= 0 && m < a.mask_rows ? a.masks + m * a.words : nullptr;
+// What is known of each row of a run.
+struct AdjustRows {
+    const uint32_t *mask[ADJUST_RUN];  // null: everything is masked
+    int length[ADJUST_RUN], prompt[ADJUST_RUN];
+    float theta[ADJUST_RUN], presence[ADJUST_RUN], frequency[ADJUST_RUN];
+    __device__ __forceinline__ void load(const Adjust &a, int64_t first, int64_t last) {
+        const int i = threadIdx.x;
+        const int64_t r = first + i;
+        __syncthreads();
+        if (r < last && i < ADJUST_RUN) {
+            const int64_t m = a.states ? a.states[r] : a.mask_rows == 1 ? 0 : r;
+            mask[i] = a.masks && m >= 0 && m < a.mask_rows ? a.masks + m * a.words : nullptr;
+            const int n = a.lengths ? a.lengths[r] : (int)a.history_len;
+            length[i] = n < 0 ? 0 : n > a.history_len ? (int)a.history_len : n;
+            prompt[i] = a.prompt_lengths ? a.prompt_lengths[r] : 0;
+            theta[i] = a.repetition ? a.repetition[r] : 1.0f;
+            presence[i] = a.presence ? a.presence[r] : 0.0f;
+            frequency[i] = a.frequency ? a.frequency[r] : 0.0f;
+        }
+        __syncthreads();
+    }
+};
+
+// A row's first tokens, one a thread, as they come from memory
+struct Recent {
+    uint32_t low, high;
+    __device__ __forceinline__ void load(const Adjust &a, const RowAt &at) {
+        low = high = 0;
+        if ((int64_t)threadIdx.x >= a.history_len) return;
+        const uint32_t *id = a.wide_ids ? (const uint32_t *)(at.of<int64_t>(a.history) + threadIdx.x) : (const uint32_t *)(at.of<int32_t>(a.history) + threadIdx.x);
+        low = id[0];
+        high = id[a.wide_ids];
+    }
+    __device__ __forceinline__ int64_t get(int wide) const { return wide ? (int64_t)((uint64_t)high << 32 | low) : (int64_t)(int32_t)low; }
+};
+
+// f(place, token) for a row's n tokens of history, over the workgroup's threads
+template <class F>
+__device__ __forceinline__ void each_history(const Adjust &a, const Recent &recent, int n, const RowAt &at, F f) {
+    if ((int)threadIdx.x < n) f((int)threadIdx.x, recent.get(a.wide_ids));
+    for (int64_t i = threadIdx.x + ADJUST_THREADS; i < n; i += ADJUST_THREADS)
+        f((int)i, a.wide_ids ? at.of<int64_t>(a.history)[i] : (int64_t)at.of<int32_t>(a.history)[i]);
 }
 
-template <class F>
-__device__ __forceinline__ void each_history(const Adjust &a, int64_t r, F f) {
-    int64_t n = a.lengths ? a.lengths[r] : a.history_len;
-    n = n < 0 ? 0 : n > a.history_len ? a.history_len : n;
-    if (a.wide_ids) {
-        const int64_t *ids = row_of<int64_t>(a.history, r, a.inner);
-        for (int64_t i = threadIdx.x; i < n; i += ADJUST_THREADS) f(i, ids[i]);
-    } else {
-        const int32_t *ids = row_of<int32_t>(a.history, r, a.inner);
-        for (int64_t i = threadIdx.x; i < n; i += ADJUST_THREADS) f(i, (int64_t)ids[i]);
+// One bit a column: those of the N columns that one load brings are the low bits of one byte.
+template <int N>
+struct Flags {
+    static constexpr int WORDS = ADJUST_THREADS * ADJUST_PACKS / 4;
+    uint32_t word[WORDS];
+    __device__ __forceinline__ void set(uint32_t k) { atomicOr(&word[k / (4 * N)], 1u << (k / N % 4 * 8 + k % N)); }
+    // the bits of columns k .. k + N, cleared
+    __device__ __forceinline__ uint32_t take(int k) {
+        uint8_t *at = (uint8_t *)word + k / N;
+        const uint32_t x = *at;
+        if (x) *at = 0;
+        return x;
+    }
+};
+
+// N elements as they are in memory, two of 16 bits in a register; 0 past the row's end
+template <class T, int N>
+struct Raw {
+    uint32_t word[N * sizeof(T) / 4];
+    __device__ __forceinline__ void load(const T *row, int col, int cols) {
+        if (col + N <= cols) {
+            __builtin_memcpy(word, row + col, sizeof word);
+        } else {
+            const int left = afresh(cols) - col;
+#pragma unroll
+            for (int i = 0; i < (int)(N * sizeof(T) / 4); i++) word[i] = 0;
+#pragma unroll
+            for (int e = 0; e < N; e++) {
+                uint32_t x = 0;
+                if (e < left) __builtin_memcpy(&x, row + col + e, sizeof(T));
+                if (sizeof(T) == 4) word[e] = x;
+                else word[e / 2] |= x << (16 * (e & 1));
+            }
+        }
+    }
+    __device__ __forceinline__ float get(int e) const {
+        const uint32_t x = sizeof(T) == 4 ? word[e] : e & 1 ? word[e / 2] >> 16 : word[e / 2] & 0xffff;
+        T v;
+        __builtin_memcpy(&v, &x, sizeof(T));
+        return (float)v;
+    }
+};
+
+// x[e] of values that stay in registers: by bits, since choices between elements would be turned into an array in memory
+template <int N>
+__device__ __forceinline__ float pick(const float *x, int e) {
+    uint32_t v = 0;
+#pragma unroll
+    for (int i = 0; i < N; i++) v |= __float_as_uint(x[i]) & (i == e ? ~0u : 0u);
+    return __uint_as_float(v);
+}
+template <int N>
+__device__ __forceinline__ void put(float *x, int e, float v) {
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const uint32_t m = i == e ? ~0u : 0u;
+        x[i] = __uint_as_float((__float_as_uint(x[i]) & ~m) | (__float_as_uint(v) & m));
     }
 }
 
-constexpr uint32_t SEEN = 1u << 31;  // of a cell: the token is in the history; below it, how often behind the prompt
+// The rows and columns of one piece of work of a launch.
+struct AdjustPart {
+    int64_t first, last;  // rows
+    int base, width;      // columns
+};
+template <class T>
+__device__ __forceinline__ AdjustPart part_of(const Adjust &a, int64_t w) {
+    AdjustPart p;
+    p.first = w / a.slices * a.run;
+    p.last = p.first + a.run < a.rows ? p.first + a.run : a.rows;
+    p.base = (int)(w % a.slices) * ADJUST_SLICE<T>;
+    p.width = a.cols - p.base < ADJUST_SLICE<T> ? a.cols - p.base : ADJUST_SLICE<T>;
+    return p;
+}
+
+// The word of a row's mask that holds column col's bit and those of its load (their number divides 32).
+__device__ __forceinline__ uint32_t mask_word(const Adjust &a, const uint32_t *mask, int col) {
+    return !a.masks ? ~0u : mask && col < a.cols ? mask[col >> 5] : 0u;
+}
 
 template <class Ti, class To>
-__global__ __launch_bounds__(ADJUST_THREADS) void adjust_kernel(Adjust a) {
+__global__ __launch_bounds__(ADJUST_THREADS, 2 * ADJUST_GROUPS) void adjust_kernel(Adjust a) {
 #pragma clang fp contract(off)
-    __shared__ uint32_t cell[ADJUST_SLICE];
-    __shared__ float extra[ADJUST_SLICE];
+    constexpr int N = Pack<Ti>::N, C = ADJUST_PACKS, NT = ADJUST_THREADS;
+    __shared__ uint32_t counts[ADJUST_SLICE<Ti>];
+    __shared__ AdjustRows known;
+    __shared__ Flags<N> seen, special;  // in the history; with a bias of the row's own
     const int t = threadIdx.x;
-    for (int64_t w = blockIdx.x; w < a.rows * a.slices; w += gridDim.x) {
-        const int64_t r = w / a.slices;
-        const int base = (int)(w % a.slices) * ADJUST_SLICE;
-        const bool past = a.history.data != nullptr, biased = a.n_biases > 0;
-        if (past || biased) {
-            __syncthreads();
-            for (int i = t; i < ADJUST_SLICE; i += ADJUST_THREADS) {
-                cell[i] = 0;
-                extra[i] = 0.0f;
-            }
-            __syncthreads();
-            if (past) {
-                const int64_t prompt = a.prompt_lengths ? a.prompt_lengths[r] : 0;
-                each_history(a, r, [&](int64_t i, int64_t id) {
-                    const int64_t k = id - base;
-                    if (k < 0 || k >= ADJUST_SLICE) return;
-                    atomicOr(&cell[k], SEEN);
-                    if (i >= prompt) atomicAdd(&cell[k], 1u);
-                });
-            }
-            // the first entry of a token sums all of its row's entries, in their order
-            for (int j = t; j < a.n_biases; j += ADJUST_THREADS) {
-                const int32_t *ids = a.bias_tokens + r * a.n_biases;
-                const float *value = a.bias_values + r * a.n_biases;
-                const int64_t k = (int64_t)ids[j] - base;
-                if (k < 0 || k >= ADJUST_SLICE) continue;
-                bool first = true;
-                for (int i = 0; i < j && first; i++) first = ids[i] != ids[j];
-                if (!first) continue;
-                float sum = value[j];
-                for (int i = j + 1; i < a.n_biases; i++)
-                    if (ids[i] == ids[j]) sum += value[i];
-                extra[k] = sum;
-            }
-            __syncthreads();
+    const bool past = a.history.data != nullptr, biased = a.n_biases > 0;
+    if (past)
+        for (int i = t; i < ADJUST_SLICE<Ti>; i += NT) counts[i] = 0;
+    for (int i = t; i < Flags<N>::WORDS; i += NT) seen.word[i] = special.word[i] = 0;
+    for (int64_t w = blockIdx.x; w < a.runs * a.slices; w += gridDim.x) {
+        const AdjustPart part = part_of<Ti>(a, w);
+        Raw<Ti, N> next[C];
+        Raw<float, N> bias[C];
+        RowAt at(part.first, a.inner), ahead = at;
+        Recent recent{};
+        if (past) recent.load(a, at);
+        uint32_t masked[C];  // the next row's
+        known.load(a, part.first, part.last);
+#pragma unroll
+        for (int c = 0; c < C; c++) {
+            const int col = part.base + (c * NT + t) * N;
+            next[c].load(at.of<Ti>(a.logits), col, a.cols);
+            masked[c] = mask_word(a, known.mask[0], col);
+            if (a.bias) bias[c].load(a.bias, col, a.cols);
+            else
+#pragma unroll
+                for (int e = 0; e < N; e++) bias[c].word[e] = 0x80000000u;  // -0: what adds nothing
         }
-        const float theta = a.repetition ? a.repetition[r] : 1.0f;
-        const float presence = a.presence ? a.presence[r] : 0.0f, frequency = a.frequency ? a.frequency[r] : 0.0f;
-        const uint32_t *mask = a.masks ? mask_row(a, r) : nullptr;
-        const Ti *in = row_of<Ti>(a.logits, r, a.inner);
-        To *out = row_of<To>(a.out, r, a.inner);
-        constexpr int N = Pack<Ti>::N;
+        for (int64_t r = part.first; r < part.last; r++, at = ahead) {
+            ahead.next(a.inner);
+            const int i = (int)(r - part.first);
+            const bool more = r + 1 < part.last;
+            Raw<Ti, N> z[C];
+            uint32_t allowed[C];
 #pragma unroll
-        for (int c = 0; c < ADJUST_EACH / N; c++) {
-            const int k = (c * ADJUST_THREADS + t) * N, col = base + k;
-            if (col >= a.cols) continue;
-            float z[N];
-            load_floats<Ti, N>(in, col, a.cols, 0.0f, z);
-            uint32_t allowed = ~0u;
-            if (a.masks) allowed = mask ? mask[col >> 5] >> (col & 31) : 0u;  // (col is a multiple of N: one word holds them)
-#pragma unroll
-            for (int e = 0; e < N; e++) {
-                float y = z[e];
+            for (int c = 0; c < C; c++) {
+                const int col = part.base + (c * NT + t) * N;
+                z[c] = next[c];
+                allowed[c] = masked[c] >> (col & 31);
+                if (more) {
+                    next[c].load(ahead.of<Ti>(a.logits), col, a.cols);
+                    masked[c] = mask_word(a, known.mask[i + 1], col);
+                }
+            }
+            const Recent tokens = recent;
+            if (past && more) recent.load(a, ahead);
+            if (past || biased) {
+                __syncthreads();  // what the last row used is clear
                 if (past) {
-                    const uint32_t seen = cell[k + e];
-                    if (seen) {
-                        y = y > 0.0f ? y / theta : y * theta;
-                        const uint32_t count = seen & ~SEEN;
-                        if (count) {
-                            y = y - frequency * (float)count;
-                            y = y - presence;
+                    const int prompt = known.prompt[i];
+                    each_history(a, tokens, known.length[i], at, [&](int i, int64_t id) {
+                        const uint64_t k = (uint64_t)(id - part.base);
+                        if (k >= (uint64_t)part.width) return;
+                        seen.set((uint32_t)k);
+                        if (i >= prompt) atomicAdd(&counts[k], 1u);
+                    });
+                }
+                for (int j = t; j < a.n_biases; j += NT) {
+                    const uint64_t k = (uint64_t)((int64_t)a.bias_tokens[r * a.n_biases + j] - part.base);
+                    if (k < (uint64_t)part.width) special.set((uint32_t)k);
+                }
+                __syncthreads();
+            }
+            To *out = at.of<To>(a.out);
+#pragma unroll
+            for (int c = 0; c < C; c++) {
+                const int k = (c * NT + t) * N, col = part.base + k;
+                if (col >= a.cols) continue;
+                float y[N];
+#pragma unroll
+                for (int e = 0; e < N; e++) y[e] = z[c].get(e);
+                if (past) {
+                    uint32_t old = seen.take(k);
+                    if (old) {
+                        const float theta = known.theta[i], presence = known.presence[i], frequency = known.frequency[i];
+#pragma unroll 1
+                        for (; old; old &= old - 1) {
+                            const int e = __ffs(old) - 1;
+                            float x = pick<N>(y, e);
+                            x = x > 0.0f ? x / theta : x * theta;
+                            const uint32_t count = counts[k + e];
+                            if (count) {
+                                counts[k + e] = 0;
+                                x = x - frequency * (float)count;
+                                x = x - presence;
+                            }
+                            put<N>(y, e, x);
                         }
                     }
                 }
-                if (a.bias) y = y + (col + e < a.cols ? a.bias[col + e] : 0.0f);
-                if (biased) y = y + extra[k + e];
-                z[e] = (allowed >> e) & 1 ? y : -INF;
+#pragma unroll
+                for (int e = 0; e < N; e++) y[e] = y[e] + bias[c].get(e);
+                if (biased && special.take(k)) {
+                    // all of the row's entries in their order; those of one column are summed first
+                    float sum[N];
+#pragma unroll
+                    for (int e = 0; e < N; e++) sum[e] = -0.0f;
+                    for (int j = 0; j < a.n_biases; j++) {
+                        const uint32_t at = (uint32_t)(a.bias_tokens[r * a.n_biases + j] - col);
+                        if (at < (uint32_t)N) {
+                            const float value = a.bias_values[r * a.n_biases + j];
+#pragma unroll
+                            for (int e = 0; e < N; e++)
+                                if (at == (uint32_t)e) sum[e] += value;
+                        }
+                    }
+#pragma unroll
+                    for (int e = 0; e < N; e++) y[e] = y[e] + sum[e];
+                }
+#pragma unroll
+                for (int e = 0; e < N; e++) y[e] = (allowed[c] >> e) & 1 ? y[e] : -INF;
+                store_floats<To, N>(out, col, a.cols, y);
             }
-            store_floats<To, N>(out, col, a.cols, z);
         }
     }
 }
 
-// dz = dy * slope, masked; the sum over rows of the masked dy for the shared bias. One workgroup takes a slice of columns
-// and a run of rows, keeps its columns' sums in registers over the run, and leaves them in the workspace; a second
-// kernel adds the runs up in their order.
+// dz = dy * slope, masked; the sum over rows of the masked dy for the shared bias: a workgroup keeps its columns' sums in
+// registers over its run of rows and leaves them in the workspace; a second kernel adds the runs up in their order.
 struct AdjustGrad {
     Adjust a;  // a.out: the gradient of the output
     Rows grad_logits;
     float *grad_bias_values, *sums;
-    int run, runs;
 };
 
 template <class Ti, class To>
-__global__ __launch_bounds__(ADJUST_THREADS) void adjust_grad_kernel(AdjustGrad g) {
+__global__ __launch_bounds__(ADJUST_THREADS, 2 * ADJUST_GROUPS) void adjust_grad_kernel(AdjustGrad g) {
     const Adjust &a = g.a;
-    __shared__ uint32_t seen[ADJUST_SLICE / 32];
+    constexpr int N = Pack<Ti>::N, C = ADJUST_PACKS, NT = ADJUST_THREADS;
+    __shared__ Flags<N> seen;
+    __shared__ AdjustRows known;
     const int t = threadIdx.x;
-    constexpr int N = Pack<Ti>::N, C = ADJUST_EACH / N;
-    for (int64_t w = blockIdx.x; w < (int64_t)g.runs * a.slices; w += gridDim.x) {
-        const int64_t first = w / a.slices * g.run, last = first + g.run < a.rows ? first + g.run : a.rows;
-        const int slice = (int)(w % a.slices), base = slice * ADJUST_SLICE;
-        const bool past = a.history.data != nullptr;
-        float sum[ADJUST_EACH] = {};
-        for (int64_t r = first; r < last; r++) {
+    const bool past = a.history.data != nullptr && g.grad_logits.data != nullptr;
+    for (int i = t; i < Flags<N>::WORDS; i += NT) seen.word[i] = 0;
+    for (int64_t w = blockIdx.x; w < a.runs * a.slices; w += gridDim.x) {
+        const AdjustPart part = part_of<Ti>(a, w);
+        Raw<To, N> next[C];
+        float sum[C][N] = {};
+        RowAt at(part.first, a.inner), ahead = at;
+        Recent recent{};
+        if (past) recent.load(a, at);
+        uint32_t masked[C];  // the next row's
+        known.load(a, part.first, part.last);
+#pragma unroll
+        for (int c = 0; c < C; c++) {
+            const int col = part.base + (c * NT + t) * N;
+            next[c].load(at.of<To>(a.out), col, a.cols);
+            masked[c] = mask_word(a, known.mask[0], col);
+        }
+        for (int64_t r = part.first; r < part.last; r++, at = ahead) {
+            ahead.next(a.inner);
+            const int i = (int)(r - part.first);
+            const bool more = r + 1 < part.last;
+            Raw<To, N> up[C];
+            uint32_t allowed[C];
+#pragma unroll
+            for (int c = 0; c < C; c++) {
+                const int col = part.base + (c * NT + t) * N;
+                up[c] = next[c];
+                allowed[c] = masked[c] >> (col & 31);
+                if (more) {
+                    next[c].load(ahead.of<To>(a.out), col, a.cols);
+                    masked[c] = mask_word(a, known.mask[i + 1], col);
+                }
+            }
+            const Recent tokens = recent;
+            if (past && more) recent.load(a, ahead);
             if (past) {
                 __syncthreads();
-                for (int i = t; i < ADJUST_SLICE / 32; i += ADJUST_THREADS) seen[i] = 0;
-                __syncthreads();
-                each_history(a, r, [&](int64_t, int64_t id) {
-                    const int64_t k = id - base;
-                    if (k >= 0 && k < ADJUST_SLICE) atomicOr(&seen[k >> 5], 1u << (k & 31));
+                each_history(a, tokens, known.length[i], at, [&](int, int64_t id) {
+                    const uint64_t k = (uint64_t)(id - part.base);
+                    if (k < (uint64_t)part.width) seen.set((uint32_t)k);
                 });
                 __syncthreads();
             }
-            const float theta = a.repetition ? a.repetition[r] : 1.0f;
-            const uint32_t *mask = a.masks ? mask_row(a, r) : nullptr;
-            const Ti *in = row_of<Ti>(a.logits, r, a.inner);
-            const To *up = row_of<To>(a.out, r, a.inner);
-            Ti *down = g.grad_logits.data ? row_of<Ti>(g.grad_logits, r, a.inner) : nullptr;
 #pragma unroll
             for (int c = 0; c < C; c++) {
-                const int k = (c * ADJUST_THREADS + t) * N, col = base + k;
+                const int k = (c * NT + t) * N, col = part.base + k;
                 if (col >= a.cols) continue;
                 float d[N];
-                load_floats<To, N>(up, col, a.cols, 0.0f, d);
-                uint32_t allowed = ~0u;
-                if (a.masks) allowed = mask ? mask[col >> 5] >> (col & 31) : 0u;
-                const uint32_t old = past ? seen[k >> 5] >> (k & 31) : 0u;
 #pragma unroll
                 for (int e = 0; e < N; e++) {
-                    d[e] = (allowed >> e) & 1 ? d[e] : 0.0f;
-                    sum[c * N + e] += d[e];
-                    if ((old >> e) & 1 && col + e < a.cols) d[e] = (float)in[col + e] > 0.0f ? d[e] / theta : d[e] * theta;
+                    d[e] = (allowed[c] >> e) & 1 ? up[c].get(e) : 0.0f;
+                    sum[c][e] += d[e];
                 }
-                if (down) store_floats<Ti, N>(down, col, a.cols, d);
+                if (!g.grad_logits.data) continue;
+                uint32_t old = past ? seen.take(k) : 0u;
+                if (old) {
+                    const float theta = known.theta[i];
+                    const Ti *in = at.of<Ti>(a.logits);
+#pragma unroll 1
+                    for (; old; old &= old - 1) {
+                        const int e = __ffs(old) - 1;
+                        const float x = pick<N>(d, e);
+                        put<N>(d, e, (float)in[col + e] > 0.0f ? x / theta : x * theta);
+                    }
+                }
+                store_floats<Ti, N>(at.of<Ti>(g.grad_logits), col, a.cols, d);
             }
-            if (g.grad_bias_values)
-                for (int j = t; j < a.n_biases; j += ADJUST_THREADS) {
+            if (g.grad_bias_values) {
+                const uint32_t *mask = known.mask[i];
+                for (int j = t; j < a.n_biases; j += NT) {
                     const int32_t id = a.bias_tokens[r * a.n_biases + j];
                     float d = 0.0f;
                     if (id < 0 || id >= a.cols) {
-                        if (slice) continue;  // (no slice holds it: the first one writes its 0)
+                        if (part.base) continue;  // (no slice holds it: the first one writes its 0)
                     } else {
-                        if (id / ADJUST_SLICE != slice) continue;
-                        if (!a.masks || (mask && (mask[id >> 5] >> (id & 31)) & 1)) d = (float)up[id];
+                        if (id < part.base || id >= part.base + part.width) continue;
+                        if (!a.masks || (mask && (mask[id >> 5] >> (id & 31)) & 1)) d = (float)at.of<To>(a.out)[id];
                     }
                     g.grad_bias_values[r * a.n_biases + j] = d;
                 }
+            }
         }
         if (g.sums)
 #pragma unroll
             for (int c = 0; c < C; c++)
-#pragma unroll
-                for (int e = 0; e < N; e++) {
-                    const int col = base + (c * ADJUST_THREADS + t) * N + e;
-                    if (col < a.cols) g.sums[w / a.slices * a.cols + col] = sum[c * N + e];
-                }
+                store_floats<float, N>(g.sums + w / a.slices * a.cols, part.base + (c * NT + t) * N, a.cols, sum[c]);
     }
 }
 
-__global__ __launch_bounds__(256) void adjust_bias_kernel(const float *sums, int runs, int cols, float *grad_bias) {
+__global__ __launch_bounds__(1024) void adjust_bias_kernel(const float *sums, int64_t runs, int cols, float *grad_bias) {
+    constexpr int PARTS = 16;
     const int col = blockIdx.x * 64 + (threadIdx.x & 63), part = threadIdx.x >> 6;
-    __shared__ float other[3][64];
+    __shared__ float other[PARTS][64];
     float s = 0.0f;
     if (col < cols)
-        for (int i = part; i < runs; i += 4) s += sums[(int64_t)i * cols + col];
-    if (part) other[part - 1][threadIdx.x & 63] = s;
+#pragma unroll 4
+        for (int64_t i = part; i < runs; i += PARTS) s += sums[i * cols + col];
+    other[part][threadIdx.x & 63] = s;
     __syncthreads();
-    if (!part && col < cols) grad_bias[col] = ((s + other[0][threadIdx.x]) + other[1][threadIdx.x]) + other[2][threadIdx.x];
+    if (part || col >= cols) return;
+    for (int i = 1; i < PARTS; i++) s += other[i][threadIdx.x];
+    grad_bias[col] = s;
 }
 
 // ---- the draw -----------------------------------------------------------------------------------------------------------
@@ -1173,6 +1375,18 @@ static zbpe_status grammar_of(const char *what, const zbpe_grammar *g, int64_t r
     return ZBPE_OK;
 }
 
+// Rows of one workgroup: as many workgroups as run at a time share the rows evenly (a second, partly filled turn would cost as
+// much as a full one), up to ADJUST_RUN rows each. More rows mean fewer loads of the shared bias, and fewer partial sums of its
+// gradient to write and add.
+template <class T>
+static void adjust_plan(int64_t rows, int cols, Adjust *a) {
+    constexpr int64_t groups = 256 * ADJUST_GROUPS;
+    a->slices = (cols + ADJUST_SLICE<T> - 1) / ADJUST_SLICE<T>;
+    const int64_t fit = (rows * a->slices + groups - 1) / groups;
+    a->run = (int)(fit < 1 ? 1 : fit > ADJUST_RUN ? ADJUST_RUN : fit);
+    a->runs = (rows + a->run - 1) / a->run;
+}
+
 static zbpe_status adjust_of(const char *what, const zbpe_adjust *p, Adjust *out) {
     if (!p) return refuse(ZBPE_INVALID_ARGUMENT, "%s: no arguments", what);
     if (p->struct_size != sizeof(zbpe_adjust)) return refuse(ZBPE_INVALID_ARGUMENT, "%s: arguments of another version", what);
@@ -1199,7 +1413,6 @@ static zbpe_status adjust_of(const char *what, const zbpe_adjust *p, Adjust *out
     a.rows = p->rows;
     a.inner = p->inner;
     a.cols = p->cols;
-    a.slices = (p->cols + ADJUST_SLICE - 1) / ADJUST_SLICE;
     a.history_len = p->history_len;
     a.lengths = p->lengths;
     a.prompt_lengths = p->prompt_lengths;
@@ -1216,17 +1429,6 @@ static zbpe_status adjust_of(const char *what, const zbpe_adjust *p, Adjust *out
     a.states = p->states;
     *out = a;
     return ZBPE_OK;
-}
-
-// Rows of one workgroup of the gradient: its columns' sums are kept over them, so more rows mean fewer partial sums to
-// write and add; fewer rows mean more workgroups. Up to 32, as long as four workgroups remain for each of the 256 CUs.
-static int adjust_run(int64_t rows, int cols) {
-    const int64_t slices = (cols + ADJUST_SLICE - 1) / ADJUST_SLICE, fit = rows * slices / 1024;
-    return (int)(fit < 1 ? 1 : fit > 32 ? 32 : fit);
-}
-static int64_t adjust_runs(int64_t rows, int cols) {
-    const int run = adjust_run(rows, cols);
-    return (rows + run - 1) / run;
 }
 
 // One row a workgroup, without a loop over rows in the kernel: what such a loop keeps in registers for the next row costs it
@@ -1339,9 +1541,10 @@ zbpe_status zbpe_adjust_logits(int device, void *stream, const zbpe_adjust *args
     if (s != ZBPE_OK || !a.rows) return s;
     OnDevice on;
     if ((s = on.go(device)) != ZBPE_OK) return s;
-    const unsigned grid = grid_of(a.rows * a.slices);
     return by_type(args->logits.dtype, [&](auto ti) {
         using T = decltype(ti);
+        adjust_plan<T>(a.rows, a.cols, &a);
+        const unsigned grid = grid_of(a.runs * a.slices);
         if (args->out.dtype == ZBPE_F32) adjust_kernel<T, float><<<grid, ADJUST_THREADS, 0, (hipStream_t)stream>>>(a);
         else adjust_kernel<T, T><<<grid, ADJUST_THREADS, 0, (hipStream_t)stream>>>(a);
         return launched(what);
@@ -1349,7 +1552,11 @@ zbpe_status zbpe_adjust_logits(int device, void *stream, const zbpe_adjust *args
 }
 
 size_t zbpe_adjust_workspace(int64_t rows, int32_t cols) {
-    return rows < 1 || cols < 1 || cols > ZBPE_MAX_VOCAB ? 0 : (size_t)adjust_runs(rows, cols) * (size_t)cols * sizeof(float);
+    if (rows < 1 || cols < 1 || cols > ZBPE_MAX_VOCAB) return 0;
+    Adjust wide{}, narrow{};
+    adjust_plan<float>(rows, cols, &wide);
+    adjust_plan<f16>(rows, cols, &narrow);
+    return (size_t)(wide.runs > narrow.runs ? wide.runs : narrow.runs) * (size_t)cols * sizeof(float);
 }
 
 zbpe_status zbpe_adjust_logits_grad(int device, void *stream, const zbpe_adjust *args, const zbpe_rows *grad_logits,
@@ -1371,12 +1578,11 @@ zbpe_status zbpe_adjust_logits_grad(int device, void *stream, const zbpe_adjust 
     if ((s = on.go(device)) != ZBPE_OK) return s;
     g.grad_bias_values = g.a.n_biases ? grad_bias_values : nullptr;
     g.sums = grad_bias ? (float *)workspace : nullptr;
-    g.run = adjust_run(g.a.rows, g.a.cols);
-    g.runs = (int)adjust_runs(g.a.rows, g.a.cols);
     if (g.a.rows && (grad_logits || grad_bias || g.grad_bias_values)) {
-        const unsigned grid = grid_of((int64_t)g.runs * g.a.slices);
         s = by_type(args->logits.dtype, [&](auto ti) {
             using T = decltype(ti);
+            adjust_plan<T>(g.a.rows, g.a.cols, &g.a);
+            const unsigned grid = grid_of(g.a.runs * g.a.slices);
             if (args->out.dtype == ZBPE_F32) adjust_grad_kernel<T, float><<<grid, ADJUST_THREADS, 0, (hipStream_t)stream>>>(g);
             else adjust_grad_kernel<T, T><<<grid, ADJUST_THREADS, 0, (hipStream_t)stream>>>(g);
             return launched(what);
@@ -1384,7 +1590,7 @@ zbpe_status zbpe_adjust_logits_grad(int device, void *stream, const zbpe_adjust 
         if (s != ZBPE_OK) return s;
     }
     if (!grad_bias) return ZBPE_OK;
-    adjust_bias_kernel<<<(unsigned)(g.a.cols + 63) / 64, 256, 0, (hipStream_t)stream>>>(g.sums, g.runs, g.a.cols, grad_bias);
+    adjust_bias_kernel<<<(unsigned)(g.a.cols + 63) / 64, 1024, 0, (hipStream_t)stream>>>(g.sums, g.a.runs, g.a.cols, grad_bias);
     return launched(what);
 }
 
