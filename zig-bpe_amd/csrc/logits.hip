@@ -26,6 +26,14 @@ __attribute__((format(printf, 2, 3))) static zbpe_status refuse(zbpe_status s, c
     return s;
 }
 
+// The same in every lane of a wave: in scalar registers.
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); }
+__device__ __forceinline__ float uniform(float x) { return __uint_as_float(uniform(__float_as_uint(x))); }
+__device__ __forceinline__ uint64_t uniform(uint64_t x) {
+    return (uint64_t)uniform((uint32_t)(x >> 32)) << 32 | uniform((uint32_t)x);
+}
+__device__ __forceinline__ double uniform(double x) { return __longlong_as_double((int64_t)uniform((uint64_t)__double_as_longlong(x))); }
+
 // ---- rows ---------------------------------------------------------------------------------------------------------------
 
 // One matrix of a launch: where row r starts.
@@ -43,15 +51,15 @@ __device__ __forceinline__ T *row_of(const Rows &m, int64_t r, int64_t per) {
 // A row's place in both levels, for walks over consecutive rows: one division for all of them.
 struct RowAt {
     int64_t outer, inner;
-    __device__ __forceinline__ RowAt(int64_t r, int64_t per) : outer(r / per), inner(r % per) {}
+    __device__ __forceinline__ RowAt(int64_t r, int64_t per) : outer((int64_t)uniform((uint64_t)(r / per))), inner((int64_t)uniform((uint64_t)(r % per))) {}
     __device__ __forceinline__ void next(int64_t per) {
         if (++inner == per) {
             inner = 0;
             outer++;
         }
     }
-    template <class T>
-    __device__ __forceinline__ T *of(const Rows &m) const { return (T *)m.data + outer * m.outer + inner * m.inner; }
+    template <class T, int SIZE = sizeof(T)>
+    __device__ __forceinline__ T *of(const Rows &m) const { return (T *)(m.data + (outer * m.outer + inner * m.inner) * SIZE); }
 };
 
 using f16 = _Float16;
@@ -60,6 +68,10 @@ using bf16 = __bf16;
 // The same number, worked with anew: what is computed from it for the ends of rows is not kept in registers through whole loops.
 __device__ __forceinline__ int afresh(int x) {
     asm volatile("" : "+s"(x));
+    return x;
+}
+__device__ __forceinline__ uint32_t afresh(uint32_t x) {  // different in every lane
+    asm volatile("" : "+v"(x));
     return x;
 }
 
@@ -98,7 +110,7 @@ __device__ __forceinline__ void store_floats(T *row, int col, int cols, const fl
         T x[N];
 #pragma unroll
         for (int e = 0; e < N; e++) x[e] = (T)z[e];
-        __builtin_memcpy(row + col, x, sizeof x);
+        __builtin_memcpy((char *)row + (uint32_t)col * (uint32_t)sizeof(T), x, sizeof x);
     } else {
         const int left = afresh(cols) - col;
 #pragma unroll
@@ -339,7 +351,7 @@ __global__ __launch_bounds__(256) void grammar_advance_kernel(Automaton g, const
 // (the bits of one load's columns in one byte, which is 0 for most loads) and how often behind the prompt. Whoever uses a bit
 // or a count clears it.
 constexpr int ADJUST_THREADS = 512, ADJUST_PACKS = 2, ADJUST_RUN = 32;
-constexpr int ADJUST_GROUPS = 3;  // on a CU at a time: 6 waves on a SIMD leave 80 registers to a thread
+constexpr int ADJUST_GROUPS = 2;  // on a CU at a time: 4 waves on a SIMD leave 128 registers to a thread
 template <class T>
 constexpr int ADJUST_SLICE = ADJUST_THREADS * ADJUST_PACKS * Pack<T>::N;
 
@@ -382,9 +394,10 @@ struct Recent {
     __device__ __forceinline__ void load(const Adjust &a, const RowAt &at) {
         low = high = 0;
         if ((int64_t)threadIdx.x >= a.history_len) return;
-        const uint32_t *id = a.wide_ids ? (const uint32_t *)(at.of<int64_t>(a.history) + threadIdx.x) : (const uint32_t *)(at.of<int32_t>(a.history) + threadIdx.x);
-        low = id[0];
-        high = id[a.wide_ids];
+        const char *ids = a.wide_ids ? at.of<char, 8>(a.history) : at.of<char, 4>(a.history);
+        const uint32_t from = threadIdx.x << (2 + a.wide_ids);
+        low = *(const uint32_t *)(ids + from);
+        high = *(const uint32_t *)(ids + (from + 4 * a.wide_ids));
     }
     __device__ __forceinline__ int64_t get(int wide) const { return wide ? (int64_t)((uint64_t)high << 32 | low) : (int64_t)(int32_t)low; }
 };
@@ -393,7 +406,7 @@ struct Recent {
 template <class F>
 __device__ __forceinline__ void each_history(const Adjust &a, const Recent &recent, int n, const RowAt &at, F f) {
     if ((int)threadIdx.x < n) f((int)threadIdx.x, recent.get(a.wide_ids));
-    for (int64_t i = threadIdx.x + ADJUST_THREADS; i < n; i += ADJUST_THREADS)
+    for (uint32_t i = afresh(threadIdx.x) + ADJUST_THREADS; i < (uint32_t)n; i += ADJUST_THREADS)
         f((int)i, a.wide_ids ? at.of<int64_t>(a.history)[i] : (int64_t)at.of<int32_t>(a.history)[i]);
 }
 
@@ -418,7 +431,7 @@ struct Raw {
     uint32_t word[N * sizeof(T) / 4];
     __device__ __forceinline__ void load(const T *row, int col, int cols) {
         if (col + N <= cols) {
-            __builtin_memcpy(word, row + col, sizeof word);
+            __builtin_memcpy(word, (const char *)row + (uint32_t)col * (uint32_t)sizeof(T), sizeof word);
         } else {
             const int left = afresh(cols) - col;
 #pragma unroll
@@ -426,7 +439,7 @@ struct Raw {
 #pragma unroll
             for (int e = 0; e < N; e++) {
                 uint32_t x = 0;
-                if (e < left) __builtin_memcpy(&x, row + col + e, sizeof(T));
+                if (e < left) __builtin_memcpy(&x, (const char *)row + ((uint32_t)col + e) * (uint32_t)sizeof(T), sizeof(T));
                 if (sizeof(T) == 4) word[e] = x;
                 else word[e / 2] |= x << (16 * (e & 1));
             }
@@ -465,9 +478,10 @@ struct AdjustPart {
 template <class T>
 __device__ __forceinline__ AdjustPart part_of(const Adjust &a, int64_t w) {
     AdjustPart p;
-    p.first = w / a.slices * a.run;
+    const int64_t run = (int64_t)uniform((uint64_t)(w / a.slices));
+    p.first = run * a.run;
     p.last = p.first + a.run < a.rows ? p.first + a.run : a.rows;
-    p.base = (int)(w % a.slices) * ADJUST_SLICE<T>;
+    p.base = (int)(w - run * a.slices) * ADJUST_SLICE<T>;
     p.width = a.cols - p.base < ADJUST_SLICE<T> ? a.cols - p.base : ADJUST_SLICE<T>;
     return p;
 }
@@ -484,6 +498,8 @@ __global__ __launch_bounds__(ADJUST_THREADS, 2 * ADJUST_GROUPS) void adjust_kern
     __shared__ uint32_t counts[ADJUST_SLICE<Ti>];
     __shared__ AdjustRows known;
     __shared__ Flags<N> seen, special;  // in the history; with a bias of the row's own
+    __shared__ int bias_token[ZBPE_MAX_BIASES];
+    __shared__ float bias_value[ZBPE_MAX_BIASES];
     const int t = threadIdx.x;
     const bool past = a.history.data != nullptr, biased = a.n_biases > 0;
     if (past)
@@ -496,6 +512,12 @@ __global__ __launch_bounds__(ADJUST_THREADS, 2 * ADJUST_GROUPS) void adjust_kern
         RowAt at(part.first, a.inner), ahead = at;
         Recent recent{};
         if (past) recent.load(a, at);
+        int own_token = -1;  // entry t of the next row's biases
+        float own_value = 0.0f;
+        if (t < a.n_biases) {
+            own_token = a.bias_tokens[part.first * a.n_biases + t];
+            own_value = a.bias_values[part.first * a.n_biases + t];
+        }
         uint32_t masked[C];  // the next row's
         known.load(a, part.first, part.last);
 #pragma unroll
@@ -526,6 +548,12 @@ __global__ __launch_bounds__(ADJUST_THREADS, 2 * ADJUST_GROUPS) void adjust_kern
             }
             const Recent tokens = recent;
             if (past && more) recent.load(a, ahead);
+            const int token = own_token;
+            const float value = own_value;
+            if (more && t < a.n_biases) {
+                own_token = a.bias_tokens[(r + 1) * a.n_biases + t];
+                own_value = a.bias_values[(r + 1) * a.n_biases + t];
+            }
             if (past || biased) {
                 __syncthreads();  // what the last row used is clear
                 if (past) {
@@ -538,8 +566,11 @@ __global__ __launch_bounds__(ADJUST_THREADS, 2 * ADJUST_GROUPS) void adjust_kern
                     });
                 }
                 for (int j = t; j < a.n_biases; j += NT) {
-                    const uint64_t k = (uint64_t)((int64_t)a.bias_tokens[r * a.n_biases + j] - part.base);
-                    if (k < (uint64_t)part.width) special.set((uint32_t)k);
+                    const int id = j < NT ? token : a.bias_tokens[r * a.n_biases + j];
+                    bias_token[j] = id;
+                    bias_value[j] = j < NT ? value : a.bias_values[r * a.n_biases + j];
+                    const uint32_t k = (uint32_t)id - (uint32_t)part.base;
+                    if (k < (uint32_t)part.width) special.set(k);
                 }
                 __syncthreads();
             }
@@ -577,14 +608,12 @@ __global__ __launch_bounds__(ADJUST_THREADS, 2 * ADJUST_GROUPS) void adjust_kern
                     float sum[N];
 #pragma unroll
                     for (int e = 0; e < N; e++) sum[e] = -0.0f;
+#pragma unroll 4
                     for (int j = 0; j < a.n_biases; j++) {
-                        const uint32_t at = (uint32_t)(a.bias_tokens[r * a.n_biases + j] - col);
-                        if (at < (uint32_t)N) {
-                            const float value = a.bias_values[r * a.n_biases + j];
+                        const uint32_t place = (uint32_t)bias_token[j] - (uint32_t)col;
+                        const float value = bias_value[j];
 #pragma unroll
-                            for (int e = 0; e < N; e++)
-                                if (at == (uint32_t)e) sum[e] += value;
-                        }
+                        for (int e = 0; e < N; e++) sum[e] += place == (uint32_t)e ? value : -0.0f;
                     }
 #pragma unroll
                     for (int e = 0; e < N; e++) y[e] = y[e] + sum[e];
@@ -609,18 +638,30 @@ template <class Ti, class To>
 __global__ __launch_bounds__(ADJUST_THREADS, 2 * ADJUST_GROUPS) void adjust_grad_kernel(AdjustGrad g) {
     const Adjust &a = g.a;
     constexpr int N = Pack<Ti>::N, C = ADJUST_PACKS, NT = ADJUST_THREADS;
-    __shared__ Flags<N> seen;
+    __shared__ Flags<N> seen, positive;  // in the history; and with a logit above 0
     __shared__ AdjustRows known;
     const int t = threadIdx.x;
     const bool past = a.history.data != nullptr && g.grad_logits.data != nullptr;
-    for (int i = t; i < Flags<N>::WORDS; i += NT) seen.word[i] = 0;
+    for (int i = t; i < Flags<N>::WORDS; i += NT) seen.word[i] = positive.word[i] = 0;
     for (int64_t w = blockIdx.x; w < a.runs * a.slices; w += gridDim.x) {
         const AdjustPart part = part_of<Ti>(a, w);
         Raw<To, N> next[C];
         float sum[C][N] = {};
         RowAt at(part.first, a.inner), ahead = at;
-        Recent recent{};
-        if (past) recent.load(a, at);
+        // tokens are loaded two rows ahead, their logits one
+        Recent recent{}, later{};
+        float logit = 0.0f;
+        auto logit_of = [&](const Recent &x, const RowAt &row) {
+            const uint64_t k = (uint64_t)(x.get(a.wide_ids) - part.base);
+            return (int64_t)t < a.history_len && k < (uint64_t)part.width ? (float)row.of<Ti>(a.logits)[part.base + (uint32_t)k] : 0.0f;
+        };
+        if (past) {
+            recent.load(a, at);
+            logit = logit_of(recent, at);
+            RowAt second = at;
+            second.next(a.inner);
+            if (part.first + 1 < part.last) later.load(a, second);
+        }
         uint32_t masked[C];  // the next row's
         known.load(a, part.first, part.last);
 #pragma unroll
@@ -646,12 +687,21 @@ __global__ __launch_bounds__(ADJUST_THREADS, 2 * ADJUST_GROUPS) void adjust_grad
                 }
             }
             const Recent tokens = recent;
-            if (past && more) recent.load(a, ahead);
+            const float z = logit;
+            if (past && more) {
+                recent = later;
+                logit = logit_of(recent, ahead);
+                RowAt second = ahead;
+                second.next(a.inner);
+                if (r + 2 < part.last) later.load(a, second);
+            }
             if (past) {
                 __syncthreads();
-                each_history(a, tokens, known.length[i], at, [&](int, int64_t id) {
+                each_history(a, tokens, known.length[i], at, [&](int place, int64_t id) {
                     const uint64_t k = (uint64_t)(id - part.base);
-                    if (k < (uint64_t)part.width) seen.set((uint32_t)k);
+                    if (k >= (uint64_t)part.width) return;
+                    seen.set((uint32_t)k);
+                    if ((place < NT ? z : (float)at.of<Ti>(a.logits)[id]) > 0.0f) positive.set((uint32_t)k);
                 });
                 __syncthreads();
             }
@@ -669,29 +719,32 @@ __global__ __launch_bounds__(ADJUST_THREADS, 2 * ADJUST_GROUPS) void adjust_grad
                 uint32_t old = past ? seen.take(k) : 0u;
                 if (old) {
                     const float theta = known.theta[i];
-                    const Ti *in = at.of<Ti>(a.logits);
+                    const uint32_t above = positive.take(k);
 #pragma unroll 1
                     for (; old; old &= old - 1) {
                         const int e = __ffs(old) - 1;
                         const float x = pick<N>(d, e);
-                        put<N>(d, e, (float)in[col + e] > 0.0f ? x / theta : x * theta);
+                        put<N>(d, e, (above >> e) & 1 ? x / theta : x * theta);
                     }
                 }
                 store_floats<Ti, N>(at.of<Ti>(g.grad_logits), col, a.cols, d);
             }
-            if (g.grad_bias_values) {
-                const uint32_t *mask = known.mask[i];
-                for (int j = t; j < a.n_biases; j += NT) {
-                    const int32_t id = a.bias_tokens[r * a.n_biases + j];
-                    float d = 0.0f;
-                    if (id < 0 || id >= a.cols) {
-                        if (part.base) continue;  // (no slice holds it: the first one writes its 0)
-                    } else {
-                        if (id < part.base || id >= part.base + part.width) continue;
-                        if (!a.masks || (mask && (mask[id >> 5] >> (id & 31)) & 1)) d = (float)at.of<To>(a.out)[id];
-                    }
-                    g.grad_bias_values[r * a.n_biases + j] = d;
+        }
+        if (g.grad_bias_values) {  // those of all rows at once, so that their loads wait together
+            const int n = (int)(part.last - part.first) * a.n_biases;
+            for (int q = t; q < n; q += NT) {
+                const int i = q / a.n_biases;
+                const int64_t r = part.first + i;
+                const int32_t id = a.bias_tokens[part.first * a.n_biases + q];
+                float d = 0.0f;
+                if (id < 0 || id >= a.cols) {
+                    if (part.base) continue;  // (no slice holds it: the first one writes its 0)
+                } else {
+                    if (id < part.base || id >= part.base + part.width) continue;
+                    const uint32_t *mask = known.mask[i];
+                    if (!a.masks || (mask && (mask[id >> 5] >> (id & 31)) & 1)) d = (float)row_of<To>(a.out, r, a.inner)[id];
                 }
+                g.grad_bias_values[part.first * a.n_biases + q] = d;
             }
         }
         if (g.sums)
@@ -739,14 +792,6 @@ __device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float(k &
 __device__ __forceinline__ uint64_t pair_of(float z, int col) { return (uint64_t)key_of(z) << 32 | (uint32_t)~col; }
 __device__ __forceinline__ float value_of(uint64_t pair) { return of_key((uint32_t)(pair >> 32)); }
 __device__ __forceinline__ int col_of(uint64_t pair) { return (int)~(uint32_t)pair; }
-
-// The same in every lane of a wave: in scalar registers.
-__device__ __forceinline__ uint32_t uniform(uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); }
-__device__ __forceinline__ float uniform(float x) { return __uint_as_float(uniform(__float_as_uint(x))); }
-__device__ __forceinline__ uint64_t uniform(uint64_t x) {
-    return (uint64_t)uniform((uint32_t)(x >> 32)) << 32 | uniform((uint32_t)x);
-}
-__device__ __forceinline__ double uniform(double x) { return __longlong_as_double((int64_t)uniform((uint64_t)__double_as_longlong(x))); }
 
 // One workgroup draws from one row, which it reads as often as the filters need (the first time from memory, then from the
 // caches: 1000 rows of 65535 floats in 122 us, 2.1 TB/s; kept in registers instead, a row leaves no room for a second
