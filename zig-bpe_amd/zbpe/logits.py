@@ -25,6 +25,7 @@ from . import _STATUS, InternalError, InvalidArgument, Merges, ZbpeError, _ptr, 
 MAX_VOCAB = 65536
 _FLOATS = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _INTS = {torch.int32: 3, torch.int64: 4}
+_KINDS = {**_FLOATS, **_INTS}
 
 # include/zbpe.h's structures, field by field ("@": native alignment, as a C compiler lays them out)
 _ROWS = "Pqqi0q"
@@ -54,7 +55,7 @@ def _check(status: int) -> None:
 
 
 def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(device.index)  # (what torch.cuda.current_stream wraps in two objects)
 
 
 def _need(ok: bool, message: str) -> None:
@@ -62,34 +63,49 @@ def _need(ok: bool, message: str) -> None:
         raise InvalidArgument(message)
 
 
+# (Checks on the way of every call make their messages only when they fail.)
+
+
 def _is_tensor(x, name: str) -> None:
-    _need(isinstance(x, torch.Tensor), f"{name} is not a tensor")
+    if not isinstance(x, torch.Tensor):
+        raise InvalidArgument(f"{name} is not a tensor")
 
 
 def _no_gradient(**named) -> None:
     for name, x in named.items():
-        _need(not isinstance(x, torch.Tensor) or not x.requires_grad, f"{name} has no gradient here: detach it")
+        if isinstance(x, torch.Tensor) and x.requires_grad:
+            raise InvalidArgument(f"{name} has no gradient here: detach it")
 
 
 class _Rows:
     """How the rows of one call are numbered: by the logits' leading axes, in two levels."""
 
-    __slots__ = ("lead", "cols", "inner", "rows", "device")
+    __slots__ = ("lead", "cols", "inner", "rows", "device", "index")
 
     def __init__(self, logits: torch.Tensor, name: str = "logits"):
         _is_tensor(logits, name)
-        _need(logits.dtype in _FLOATS, f"{name} is {logits.dtype} (float32, float16 or bfloat16)")
-        _need(logits.dim() >= 1, f"{name} has no axis of columns")
+        if logits.dtype not in _FLOATS:
+            raise InvalidArgument(f"{name} is {logits.dtype} (float32, float16 or bfloat16)")
+        if not (logits.dim() >= 1):
+            raise InvalidArgument(f"{name} has no axis of columns")
         self.lead, self.cols = logits.shape[:-1], logits.shape[-1]
-        _need(1 <= self.cols <= MAX_VOCAB, f"{name} has {self.cols} columns (1 to {MAX_VOCAB})")
-        _need(logits.is_cuda, f"{name} is on {logits.device}, not on a GPU")
+        if not (1 <= self.cols <= MAX_VOCAB):
+            raise InvalidArgument(f"{name} has {self.cols} columns (1 to {MAX_VOCAB})")
+        if not (logits.is_cuda):
+            raise InvalidArgument(f"{name} is on {logits.device}, not on a GPU")
         self.device = logits.device
+        self.index = self.device.index
         self.rows = self.lead.numel()
         self.inner = max(self.lead[-1], 1) if self.lead else 1
 
     def matrix(self, t: torch.Tensor, keep: list):
         """(pointer, outer stride, inner stride, dtype) of a [*lead, n] tensor, copied only when two strides do not say it."""
         n = t.shape[-1]
+        if t.is_contiguous():
+            return (t.data_ptr(), self.inner * n, n, _KINDS.get(t.dtype, 0))
+        if t.dim() == 2 and t.stride(1) == 1 and t.numel():
+            step = t.stride(0)
+            return (t.data_ptr(), self.inner * step, step, _KINDS.get(t.dtype, 0))
         if t.dim() != 3:
             try:
                 t = t.view(-1, self.inner, n) if t.numel() else t
@@ -98,33 +114,41 @@ class _Rows:
         if t.numel() and n > 1 and t.stride(-1) != 1:
             t = t.contiguous()
         keep.append(t)
-        kind = _FLOATS.get(t.dtype, _INTS.get(t.dtype, 0))
+        kind = _KINDS.get(t.dtype, 0)
         if not t.numel():
             return (t.data_ptr(), n, n, kind)
         return (t.data_ptr(), t.stride(0), t.stride(1), kind)
 
     def on(self, t: torch.Tensor, name: str) -> None:
         _is_tensor(t, name)
-        _need(t.device == self.device, f"{name} is on {t.device}, the logits are on {self.device}")
+        if t.device != self.device:
+            raise InvalidArgument(f"{name} is on {t.device}, the logits are on {self.device}")
 
     def per_row(self, x, name: str, dtype: torch.dtype, keep: list) -> int:
         """Pointer of one value a row; a number stands for all rows, None for the default."""
         if x is None:
             return 0
         if not isinstance(x, torch.Tensor):
-            _need(isinstance(x, (int, float)), f"{name} is neither a tensor nor a number")
+            if not isinstance(x, (int, float)):
+                raise InvalidArgument(f"{name} is neither a tensor nor a number")
             x = torch.full(self.lead, x, dtype=dtype, device=self.device)
+        elif x.dtype == dtype and x.shape == self.lead and x.get_device() == self.index and x.is_contiguous():
+            return x.data_ptr()  # (the usual case; the caller holds it)
         self.on(x, name)
-        _need(x.dtype == dtype, f"{name} is {x.dtype} ({dtype})")
-        _need(x.shape == self.lead, f"{name} has shape {tuple(x.shape)}, the rows are {tuple(self.lead)}")
+        if x.dtype != dtype:
+            raise InvalidArgument(f"{name} is {x.dtype} ({dtype})")
+        if x.shape != self.lead:
+            raise InvalidArgument(f"{name} has shape {tuple(x.shape)}, the rows are {tuple(self.lead)}")
         x = x.contiguous()
         keep.append(x)
         return x.data_ptr()
 
     def tokens(self, x: torch.Tensor, name: str, keep: list):
         self.on(x, name)
-        _need(x.dtype in _INTS, f"{name} is {x.dtype} (int32 or int64)")
-        _need(x.shape == self.lead, f"{name} has shape {tuple(x.shape)}, the rows are {tuple(self.lead)}")
+        if x.dtype not in _INTS:
+            raise InvalidArgument(f"{name} is {x.dtype} (int32 or int64)")
+        if x.shape != self.lead:
+            raise InvalidArgument(f"{name} has shape {tuple(x.shape)}, the rows are {tuple(self.lead)}")
         x = x.contiguous()
         keep.append(x)
         return x.data_ptr(), _INTS[x.dtype]
@@ -148,8 +172,8 @@ def token_bytes(merges, vocab_size: Optional[int] = None):
     a = _triples(merges)
     if vocab_size is None:
         vocab_size = max(vocabStart, int(a[:, 2].max()) + 1 if len(a) else 0)
-    _need(isinstance(vocab_size, (int, np.integer)) and vocabStart <= vocab_size <= MAX_VOCAB,
-          f"vocab_size is {vocab_size} ({vocabStart} to {MAX_VOCAB})")
+    if not (isinstance(vocab_size, (int, np.integer)) and vocabStart <= vocab_size <= MAX_VOCAB):
+        raise InvalidArgument(f"vocab_size is {vocab_size} ({vocabStart} to {MAX_VOCAB})")
     L = _library()
     triples = a if len(a) else np.zeros(3, np.uint16)
     offsets, n = np.zeros(vocab_size + 1, np.uint32), ctypes.c_size_t(0)
@@ -169,7 +193,8 @@ class Vocabulary:
         offsets, data = token_bytes(merges, vocab_size)
         self.size = len(offsets) - 1
         self.end_token = -1 if end_token is None else int(end_token)
-        _need(end_token is None or 0 <= self.end_token < self.size, f"end_token is {end_token}, the vocabulary has {self.size} tokens")
+        if not (end_token is None or 0 <= self.end_token < self.size):
+            raise InvalidArgument(f"end_token is {end_token}, the vocabulary has {self.size} tokens")
         self.words = (self.size + 31) // 32
         self.device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
         if self.device.type == "cuda" and self.device.index is None:
@@ -207,18 +232,23 @@ class Grammar:
         _need(isinstance(vocabulary, Vocabulary), "vocabulary is not a Vocabulary")
         device = vocabulary.device
         next = torch.as_tensor(next)
-        _need(next.dim() == 2 and next.shape[1] == 256, f"next has shape {tuple(next.shape)} (states, 256)")
+        if not (next.dim() == 2 and next.shape[1] == 256):
+            raise InvalidArgument(f"next has shape {tuple(next.shape)} (states, 256)")
         n = next.shape[0]
-        _need(n < 1 << 23, f"{n} states (fewer than 2^23)")
-        _need(not next.is_floating_point() and not next.is_complex() and next.dtype != torch.bool, f"next is {next.dtype} (whole numbers)")
+        if not (n < 1 << 23):
+            raise InvalidArgument(f"{n} states (fewer than 2^23)")
+        if next.is_floating_point() or next.is_complex() or next.dtype == torch.bool:
+            raise InvalidArgument(f"next is {next.dtype} (whole numbers)")
         if next.dtype != torch.int32:
             next = torch.where((next < 0) | (next >= n), -1, next).to(torch.int32)
         self.next = next.to(device).contiguous()
         self.accepting = None
         if accepting is not None:
             accepting = torch.as_tensor(accepting)
-            _need(accepting.dtype in (torch.bool, torch.uint8), f"accepting is {accepting.dtype} (bool)")
-            _need(accepting.shape == (n,), f"accepting has shape {tuple(accepting.shape)}, there are {n} states")
+            if not (accepting.dtype in (torch.bool, torch.uint8)):
+                raise InvalidArgument(f"accepting is {accepting.dtype} (bool)")
+            if accepting.shape != (n,):
+                raise InvalidArgument(f"accepting has shape {tuple(accepting.shape)}, there are {n} states")
             self.accepting = accepting.to(device).contiguous()
         self.vocabulary, self.states = vocabulary, n
 
@@ -229,8 +259,10 @@ class Grammar:
 
     def _vector(self, x: torch.Tensor, name: str) -> torch.Tensor:
         _is_tensor(x, name)
-        _need(x.device == self.next.device, f"{name} is on {x.device}, the grammar is on {self.next.device}")
-        _need(x.dtype == torch.int32, f"{name} is {x.dtype} (int32)")
+        if x.device != self.next.device:
+            raise InvalidArgument(f"{name} is on {x.device}, the grammar is on {self.next.device}")
+        if x.dtype != torch.int32:
+            raise InvalidArgument(f"{name} is {x.dtype} (int32)")
         return x.contiguous()
 
     def masks(self, states: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -245,8 +277,8 @@ class Grammar:
             out = torch.empty(shape, dtype=torch.int32, device=device)
         else:
             _is_tensor(out, "out")
-            _need(out.dtype == torch.int32 and out.shape == shape and out.device == device and out.is_contiguous(),
-                  f"out is not a packed int32 tensor of shape {tuple(shape)} on {device}")
+            if not (out.dtype == torch.int32 and out.shape == shape and out.device == device and out.is_contiguous()):
+                raise InvalidArgument(f"out is not a packed int32 tensor of shape {tuple(shape)} on {device}")
         rows = self.states if states is None else states.numel()
         _check(_library().zbpe_grammar_masks(device.index, _stream(device), self._packed(),
                                              None if states is None else states.data_ptr(), rows, out.data_ptr()))
@@ -256,7 +288,8 @@ class Grammar:
         """The states after `tokens` (int32 both, of one shape): -1 where the grammar refuses the token. A negative token
         leaves its state as it is."""
         states, tokens = self._vector(states, "states"), self._vector(tokens, "tokens")
-        _need(states.shape == tokens.shape, f"states have shape {tuple(states.shape)}, tokens {tuple(tokens.shape)}")
+        if states.shape != tokens.shape:
+            raise InvalidArgument(f"states have shape {tuple(states.shape)}, tokens {tuple(tokens.shape)}")
         out = torch.empty_like(states)
         device = self.next.device
         _check(_library().zbpe_grammar_advance(device.index, _stream(device), self._packed(), states.data_ptr(), tokens.data_ptr(),
@@ -287,18 +320,21 @@ def _pack_adjust(at: _Rows, logits: torch.Tensor, out: torch.Tensor, x: _Terms, 
     history, length = _NO_ROWS, 0
     if x.history is not None:
         at.on(x.history, "history")
-        _need(x.history.dtype in _INTS, f"history is {x.history.dtype} (int32 or int64)")
-        _need(x.history.shape[:-1] == at.lead and x.history.dim() == len(at.lead) + 1,
-              f"history has shape {tuple(x.history.shape)}, the rows are {tuple(at.lead)}")
+        if x.history.dtype not in _INTS:
+            raise InvalidArgument(f"history is {x.history.dtype} (int32 or int64)")
+        if not (x.history.shape[:-1] == at.lead and x.history.dim() == len(at.lead) + 1):
+            raise InvalidArgument(f"history has shape {tuple(x.history.shape)}, the rows are {tuple(at.lead)}")
         length = x.history.shape[-1]
         history = at.matrix(x.history, keep)
     else:
         for name in ("lengths", "prompt_lengths", "repetition", "presence", "frequency"):
-            _need(getattr(x, name) is None, f"{name} without a history")
+            if getattr(x, name) is not None:
+                raise InvalidArgument(f"{name} without a history")
     bias = 0
     if x.bias is not None:
         at.on(x.bias, "bias")
-        _need(x.bias.dtype == torch.float32 and x.bias.shape == (at.cols,), f"bias is not float32 of {at.cols} values")
+        if not (x.bias.dtype == torch.float32 and x.bias.shape == (at.cols,)):
+            raise InvalidArgument(f"bias is not float32 of {at.cols} values")
         t = x.bias.contiguous()
         keep.append(t)
         bias = t.data_ptr()
@@ -308,8 +344,10 @@ def _pack_adjust(at: _Rows, logits: torch.Tensor, out: torch.Tensor, x: _Terms, 
         for name, kind in (("bias_tokens", torch.int32), ("bias_values", torch.float32)):
             t = getattr(x, name)
             at.on(t, name)
-            _need(t.dtype == kind, f"{name} is {t.dtype} ({kind})")
-            _need(t.dim() == len(at.lead) + 1 and t.shape[:-1] == at.lead, f"{name} has shape {tuple(t.shape)}, the rows are {tuple(at.lead)}")
+            if t.dtype != kind:
+                raise InvalidArgument(f"{name} is {t.dtype} ({kind})")
+            if not (t.dim() == len(at.lead) + 1 and t.shape[:-1] == at.lead):
+                raise InvalidArgument(f"{name} has shape {tuple(t.shape)}, the rows are {tuple(at.lead)}")
         n_biases = x.bias_tokens.shape[-1]
         _need(x.bias_values.shape == x.bias_tokens.shape, "bias_tokens and bias_values have different shapes")
         t, v = x.bias_tokens.contiguous(), x.bias_values.contiguous()
@@ -318,15 +356,18 @@ def _pack_adjust(at: _Rows, logits: torch.Tensor, out: torch.Tensor, x: _Terms, 
     masks, mask_words, mask_rows, states = 0, 0, 0, 0
     if x.masks is not None:
         at.on(x.masks, "masks")
-        _need(x.masks.dtype == torch.int32, f"masks are {x.masks.dtype} (int32)")
-        _need(x.masks.dim() >= 1 and x.masks.shape[-1] >= (at.cols + 31) // 32,
-              f"masks of shape {tuple(x.masks.shape)} are too narrow for {at.cols} columns")
-        _need(x.masks.numel() > 0 or at.rows == 0, f"masks of shape {tuple(x.masks.shape)} have no rows")
+        if x.masks.dtype != torch.int32:
+            raise InvalidArgument(f"masks are {x.masks.dtype} (int32)")
+        if not (x.masks.dim() >= 1 and x.masks.shape[-1] >= (at.cols + 31) // 32):
+            raise InvalidArgument(f"masks of shape {tuple(x.masks.shape)} are too narrow for {at.cols} columns")
+        if not (x.masks.numel() > 0 or at.rows == 0):
+            raise InvalidArgument(f"masks of shape {tuple(x.masks.shape)} have no rows")
         t = x.masks.contiguous()
         keep.append(t)
         masks, mask_words, mask_rows = t.data_ptr(), t.shape[-1], t.shape[:-1].numel()
         if x.states is None:
-            _need(t.shape[:-1] == at.lead or mask_rows == 1, f"masks of shape {tuple(t.shape)}, the rows are {tuple(at.lead)}")
+            if not (t.shape[:-1] == at.lead or mask_rows == 1):
+                raise InvalidArgument(f"masks of shape {tuple(t.shape)}, the rows are {tuple(at.lead)}")
         else:
             states = at.per_row(x.states, "states", torch.int32, keep)
     else:
@@ -405,11 +446,9 @@ def adjust_logits(logits: torch.Tensor, *, history: Optional[torch.Tensor] = Non
     if out is not None:
         _need(not learns, "out goes without gradients")
         _is_tensor(out, "out")
-        _need(out.shape == logits.shape and out.device == logits.device and out.dtype in (logits.dtype, torch.float32),
-              f"out is not {logits.dtype} or float32 of shape {tuple(logits.shape)} on {logits.device}")
-        at, probe = _Rows(logits), []
-        at.matrix(out, probe)
-        _need(probe[0].data_ptr() == out.data_ptr(), "out has strides that its rows cannot be written by")
+        if not (out.shape == logits.shape and out.device == logits.device and out.dtype in (logits.dtype, torch.float32)):
+            raise InvalidArgument(f"out is not {logits.dtype} or float32 of shape {tuple(logits.shape)} on {logits.device}")
+        _need(_Rows(logits).matrix(out, [])[0] == out.data_ptr(), "out has strides that its rows cannot be written by")
         return _adjust(logits, out, x)
     if learns:
         return _Adjust.apply(logits, bias, bias_values, x, logits.dtype)
