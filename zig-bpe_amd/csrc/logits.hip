@@ -388,14 +388,14 @@ struct AdjustRows {
     }
 };
 
-// A row's first tokens, one a thread, as they come from memory
+// A token of a row's history, as it comes from memory: that at the thread's place, if no other is named
 struct Recent {
     uint32_t low, high;
-    __device__ __forceinline__ void load(const Adjust &a, const RowAt &at) {
+    __device__ __forceinline__ void load(const Adjust &a, const RowAt &at, uint32_t place = threadIdx.x) {
         low = high = 0;
-        if ((int64_t)threadIdx.x >= a.history_len) return;
+        if ((int64_t)place >= a.history_len) return;
         const char *ids = a.wide_ids ? at.of<char, 8>(a.history) : at.of<char, 4>(a.history);
-        const uint32_t from = threadIdx.x << (2 + a.wide_ids);
+        const uint64_t from = (uint64_t)place << (2 + a.wide_ids);
         low = *(const uint32_t *)(ids + from);
         high = *(const uint32_t *)(ids + (from + 4 * a.wide_ids));
     }
@@ -406,8 +406,15 @@ struct Recent {
 template <class F>
 __device__ __forceinline__ void each_history(const Adjust &a, const Recent &recent, int n, const RowAt &at, F f) {
     if ((int)threadIdx.x < n) f((int)threadIdx.x, recent.get(a.wide_ids));
-    for (uint32_t i = afresh(threadIdx.x) + ADJUST_THREADS; i < (uint32_t)n; i += ADJUST_THREADS)
-        f((int)i, a.wide_ids ? at.of<int64_t>(a.history)[i] : (int64_t)at.of<int32_t>(a.history)[i]);
+    constexpr int AHEAD = 4;
+    for (uint32_t i = afresh(threadIdx.x) + ADJUST_THREADS; i < (uint32_t)n; i += AHEAD * ADJUST_THREADS) {
+        Recent x[AHEAD];
+#pragma unroll
+        for (int q = 0; q < AHEAD; q++) x[q].load(a, at, i + q * ADJUST_THREADS);
+#pragma unroll
+        for (int q = 0; q < AHEAD; q++)
+            if (i + q * ADJUST_THREADS < (uint32_t)n) f((int)(i + q * ADJUST_THREADS), x[q].get(a.wide_ids));
+    }
 }
 
 // One bit a column: those of the N columns that one load brings are the low bits of one byte.
@@ -1266,10 +1273,10 @@ __device__ __forceinline__ int64_t token_of(const Logprobs &a, int64_t r) {
     return a.wide_ids ? ((const int64_t *)a.tokens)[r] : (int64_t)((const int32_t *)a.tokens)[r];
 }
 
-// One pass with a running maximum and sum. TPR threads go over one row.
+// One pass with a running maximum and sum. TPR threads go over one row, AHEAD loads of 16 bytes each at a time.
 template <class T, int TPR>
 __global__ __launch_bounds__(256) void logprobs_kernel(Logprobs a) {
-    constexpr int N = Pack<T>::N, PER = 256 / TPR;
+    constexpr int N = Pack<T>::N, PER = 256 / TPR, AHEAD = 4;
     __shared__ float maxima[4], sums[4];
     const int t = threadIdx.x % TPR;
     for (int64_t r0 = blockIdx.x * (int64_t)PER; r0 < a.rows; r0 += gridDim.x * (int64_t)PER) {
@@ -1279,19 +1286,35 @@ __global__ __launch_bounds__(256) void logprobs_kernel(Logprobs a) {
         const float inverse = 1.0f / temperature, scale = inverse * LOG2E;
         const T *row = on ? row_of<T>(a.logits, r, a.inner) : nullptr;
         float m = -INF, s = 0.0f;
-        if (on)
-            for (int col = t * N; col < a.cols; col += TPR * N) {
+        auto add = [&](const float *z, int n) {
+            float more = m;
+#pragma unroll
+            for (int e = 0; e < n; e++) more = fmaxf(more, z[e]);
+            const float from = more == -INF ? 0.0f : more;  // (nothing yet above -inf: the exponentials are 0, not NaN)
+            s *= __builtin_amdgcn_exp2f((m - from) * scale);
+#pragma unroll
+            for (int e = 0; e < n; e++) s += __builtin_amdgcn_exp2f((z[e] - from) * scale);
+            m = more;
+        };
+        if (on) {
+            int col = t * N;
+#pragma unroll 1
+            for (; col + ((AHEAD - 1) * TPR + 1) * N <= a.cols; col += AHEAD * TPR * N) {
+                Pack<T> x[AHEAD];
+#pragma unroll
+                for (int i = 0; i < AHEAD; i++) x[i] = load_pack(row + col + i * TPR * N);
+                float z[AHEAD * N];
+#pragma unroll
+                for (int i = 0; i < AHEAD * N; i++) z[i] = (float)x[i / N].v[i % N];
+                add(z, AHEAD * N);
+            }
+#pragma unroll 1
+            for (; col < a.cols; col += TPR * N) {
                 float z[N];
                 load_floats<T, N>(row, col, a.cols, -INF, z);
-                float more = m;
-#pragma unroll
-                for (int e = 0; e < N; e++) more = fmaxf(more, z[e]);
-                const float from = more == -INF ? 0.0f : more;  // (nothing yet above -inf: the exponentials are 0, not NaN)
-                s *= __builtin_amdgcn_exp2f((m - from) * scale);
-#pragma unroll
-                for (int e = 0; e < N; e++) s += __builtin_amdgcn_exp2f((z[e] - from) * scale);
-                m = more;
+                add(z, N);
             }
+        }
         float top = wave_max(m);
         s = wave_sum(s * __builtin_amdgcn_exp2f((m - (top == -INF ? 0.0f : top)) * scale));
         if (TPR > 64) {
@@ -1325,7 +1348,7 @@ template <class T>
 __global__ __launch_bounds__(256) void logprobs_grad_kernel(Logprobs a, int slices) {
     constexpr int N = Pack<T>::N, EACH = 2 * N;
     for (int64_t w = blockIdx.x; w < a.rows * slices; w += gridDim.x) {
-        const int64_t r = w / slices;
+        const int64_t r = a.rows - 1 - w / slices;  // what the forward pass read last may still be in the cache
         const int64_t token = token_of(a, r);
         const float temperature = a.temperature ? a.temperature[r] : 1.0f;
         const float inverse = 1.0f / temperature, scale = inverse * LOG2E;
