@@ -88,6 +88,34 @@ __device__ __forceinline__ Pack<T> load_pack(const T *p) {
     __builtin_memcpy(&x, p, sizeof x);
     return x;
 }
+// N elements as they are in memory, two of 16 bits in a register; 0 past the row's end
+template <class T, int N>
+struct Raw {
+    uint32_t word[N * sizeof(T) / 4];
+    __device__ __forceinline__ void load(const T *row, int col, int cols) {
+        if (col + N <= cols) {
+            __builtin_memcpy(word, (const char *)row + (uint32_t)col * (uint32_t)sizeof(T), sizeof word);
+        } else {
+            const int left = afresh(cols) - col;
+#pragma unroll
+            for (int i = 0; i < (int)(N * sizeof(T) / 4); i++) word[i] = 0;
+#pragma unroll
+            for (int e = 0; e < N; e++) {
+                uint32_t x = 0;
+                if (e < left) __builtin_memcpy(&x, (const char *)row + ((uint32_t)col + e) * (uint32_t)sizeof(T), sizeof(T));
+                if (sizeof(T) == 4) word[e] = x;
+                else word[e / 2] |= x << (16 * (e & 1));
+            }
+        }
+    }
+    __device__ __forceinline__ float get(int e) const {
+        const uint32_t x = sizeof(T) == 4 ? word[e] : e & 1 ? word[e / 2] >> 16 : word[e / 2] & 0xffff;
+        T v;
+        __builtin_memcpy(&v, &x, sizeof(T));
+        return (float)v;
+    }
+};
+
 // N consecutive elements as floats; those past `cols` become `fill`.
 template <class T, int N>
 __device__ __forceinline__ void load_floats(const T *row, int col, int cols, float fill, float *z) {
@@ -429,34 +457,6 @@ struct Flags {
         const uint32_t x = *at;
         if (x) *at = 0;
         return x;
-    }
-};
-
-// N elements as they are in memory, two of 16 bits in a register; 0 past the row's end
-template <class T, int N>
-struct Raw {
-    uint32_t word[N * sizeof(T) / 4];
-    __device__ __forceinline__ void load(const T *row, int col, int cols) {
-        if (col + N <= cols) {
-            __builtin_memcpy(word, (const char *)row + (uint32_t)col * (uint32_t)sizeof(T), sizeof word);
-        } else {
-            const int left = afresh(cols) - col;
-#pragma unroll
-            for (int i = 0; i < (int)(N * sizeof(T) / 4); i++) word[i] = 0;
-#pragma unroll
-            for (int e = 0; e < N; e++) {
-                uint32_t x = 0;
-                if (e < left) __builtin_memcpy(&x, (const char *)row + ((uint32_t)col + e) * (uint32_t)sizeof(T), sizeof(T));
-                if (sizeof(T) == 4) word[e] = x;
-                else word[e / 2] |= x << (16 * (e & 1));
-            }
-        }
-    }
-    __device__ __forceinline__ float get(int e) const {
-        const uint32_t x = sizeof(T) == 4 ? word[e] : e & 1 ? word[e / 2] >> 16 : word[e / 2] & 0xffff;
-        T v;
-        __builtin_memcpy(&v, &x, sizeof(T));
-        return (float)v;
     }
 };
 
@@ -1344,11 +1344,18 @@ __global__ __launch_bounds__(256) void logprobs_kernel(Logprobs a) {
     }
 }
 
+// One slice of columns (blockIdx.y) of one row after another.
 template <class T>
-__global__ __launch_bounds__(256) void logprobs_grad_kernel(Logprobs a, int slices) {
-    constexpr int N = Pack<T>::N, EACH = 2 * N;
-    for (int64_t w = blockIdx.x; w < a.rows * slices; w += gridDim.x) {
-        const int64_t r = a.rows - 1 - w / slices;  // what the forward pass read last may still be in the cache
+__global__ __launch_bounds__(256) void logprobs_grad_kernel(Logprobs a) {
+    constexpr int N = Pack<T>::N, C = 2;
+    const int first = blockIdx.y * 256 * C * N + threadIdx.x * N;
+    for (int64_t i = blockIdx.x; i < a.rows; i += gridDim.x) {
+        const int64_t r = a.rows - 1 - i;  // what the forward pass read last may still be in the cache
+        const T *row = row_of<T>(a.logits, r, a.inner);
+        T *out = row_of<T>(a.grad_logits, r, a.inner);
+        Raw<T, N> x[C];
+#pragma unroll
+        for (int c = 0; c < C; c++) x[c].load(row, first + c * 256 * N, a.cols);
         const int64_t token = token_of(a, r);
         const float temperature = a.temperature ? a.temperature[r] : 1.0f;
         const float inverse = 1.0f / temperature, scale = inverse * LOG2E;
@@ -1356,17 +1363,14 @@ __global__ __launch_bounds__(256) void logprobs_grad_kernel(Logprobs a, int slic
         const bool scored = token >= 0 && s != 0.0f;
         const float g = scored ? a.grad[r] * inverse : 0.0f;
         const float less = token >= a.cols ? __builtin_nanf("") : g / s;
-        const T *row = row_of<T>(a.logits, r, a.inner);
-        T *out = row_of<T>(a.grad_logits, r, a.inner);
 #pragma unroll
-        for (int c = 0; c < 2; c++) {
-            const int col = (int)(w % slices) * 256 * EACH + (c * 256 + (int)threadIdx.x) * N;
+        for (int c = 0; c < C; c++) {
+            const int col = first + c * 256 * N;
             if (col >= a.cols) continue;
             float z[N];
-            load_floats<T, N>(row, col, a.cols, 0.0f, z);
 #pragma unroll
             for (int e = 0; e < N; e++) {
-                const float d = scored ? -less * __builtin_amdgcn_exp2f((z[e] - top) * scale) : 0.0f;
+                const float d = scored ? -less * __builtin_amdgcn_exp2f((x[c].get(e) - top) * scale) : 0.0f;
                 z[e] = col + e == token ? g + d : d;
             }
             store_floats<T, N>(out, col, a.cols, z);
@@ -1711,7 +1715,7 @@ zbpe_status zbpe_token_logprobs_grad(int device, void *stream, const zbpe_logpro
     return by_type(args->logits.dtype, [&](auto ti) {
         using T = decltype(ti);
         const int each = 512 * Pack<T>::N, slices = (a.cols + each - 1) / each;
-        logprobs_grad_kernel<T><<<grid_of(a.rows * slices), 256, 0, (hipStream_t)stream>>>(a, slices);
+        logprobs_grad_kernel<T><<<dim3(grid_of(a.rows), (unsigned)slices), 256, 0, (hipStream_t)stream>>>(a);
         return launched(what);
     });
 }
