@@ -206,7 +206,7 @@ __device__ __forceinline__ int walk(const Automaton &g, int s, uint32_t at, uint
 // states follow, -1: refused). The bits return to the order of ids in shared memory.
 template <int NT>
 __global__ __launch_bounds__(NT) void grammar_masks_kernel(Automaton g, const int32_t *states, int64_t rows, uint32_t *masks, int slices, int per) {
-    constexpr int ROWS = 8, SLICES = ZBPE_MAX_VOCAB / INDEX_SLICE, SLICE_WORDS = INDEX_SLICE / 32;
+    constexpr int ROWS = 4, SLICES = ZBPE_MAX_VOCAB / INDEX_SLICE, SLICE_WORDS = INDEX_SLICE / 32;
     __shared__ int next[ROWS][256];
     __shared__ int place[ROWS];  // the states of these rows
     __shared__ uint32_t live[8], turns[2][4];  // the bytes that the state takes; the classes with a byte that changes it
