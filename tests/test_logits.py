@@ -386,6 +386,28 @@ def test_masks_of_every_state_of_a_large_automaton():
 
 
 @gpu
+def test_masks_of_many_rows_over_several_slices():
+    """rows enough that a workgroup takes several slices of ids; tokens longer than the index holds; states with many successors"""
+    rng = np.random.default_rng(11)
+    size, end = 20000, 12345
+    merges = some_merges(size, rng, ALPHABET, most=40, skip=0.02)
+    table, accepting = some_automaton(60, rng, ALPHABET)
+    table[0, ALPHABET] = 0
+    table[1, ALPHABET] = np.arange(len(ALPHABET)) + 1
+    accepting[0] = True
+    tokens = tokens_of(merges, size)
+    assert max(len(t) for t in tokens if t) > 30
+    g = zbpe.Grammar(zbpe.Vocabulary(np.array(merges), size, end), cuda(table), cuda(accepting))
+    few = np.array([0, 1, 2, 59, -1, 60], np.int32)
+    want = np.stack([allowed_after(table, accepting, tokens, end, int(s)) for s in few])
+    for rows in (len(few), 400, 1500, 3000, 6000):
+        pick = np.concatenate([np.arange(len(few)), rng.integers(0, len(few), rows - len(few))])
+        got = g.masks(cuda(few[pick]))
+        np.testing.assert_array_equal(unpack(got[:len(few)], size), want)
+        assert torch.equal(got, got[:len(few)][torch.from_numpy(pick).cuda()])
+
+
+@gpu
 def test_grammar_edges_and_refusals():
     v = zbpe.Vocabulary([], 256)
     g = zbpe.Grammar(v, torch.zeros(0, 256, dtype=torch.int32))  # no states: nothing is allowed, nothing moves
@@ -622,6 +644,35 @@ def test_adjust_gradients(rows, cols, kind):
         g1 = {k: v.detach().requires_grad_(k == name) if v.is_floating_point() else v for k, v in g.items()}
         leaf = z1 if i == 0 else g1[name]
         assert torch.equal(torch.autograd.grad(zbpe.adjust_logits(z1, **g1), leaf, up.cuda())[0], got[i])
+
+
+@gpu
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("history, biases, wide", [(1300, 3, True), (2600, 700, False)])
+def test_adjust_runs_of_rows(kind, history, biases, wide):
+    """several rows and slices for a workgroup, histories and biases longer than one load of it, rows cut out of a wider tensor"""
+    lead, cols = (20, 15), 9001
+    z, x = adjust_case(300, cols, history, history=history, biases=biases, kind=kind, wide=wide)
+    up = torch.from_numpy(np.random.default_rng(2).standard_normal((300, cols))).to(kind)
+    y, bound, dz, db, dv, db_bound = adjust_oracle(z, x, up)
+    g = {k: v.view(*lead, *v.shape[1:]) if k not in ("bias", "masks") else v for k, v in to_gpu(x).items()}
+    whole = torch.zeros(20, 17, cols, dtype=kind, device="cuda")
+    whole[:, 1:16] = z.view(*lead, cols).cuda()
+    zg = whole[:, 1:16].requires_grad_()
+    g["bias"].requires_grad_()
+    g["bias_values"].requires_grad_()
+    out = zbpe.adjust_logits(zg, **g)
+    relative, least = half_step(kind)
+    close(out.view(300, cols), y, bound + (np.where(np.isfinite(y), np.abs(y), 0) + bound) * relative + least)
+    got = torch.autograd.grad(out, [zg, g["bias"], g["bias_values"]], up.view(*lead, cols).cuda())
+    close(got[0].reshape(300, cols), dz, np.abs(dz) * (relative + 2 * U) + least)
+    close(got[1], db, db_bound)
+    close(got[2].reshape(300, -1), dv, np.abs(dv) * 0)
+    # in place, and nothing beside the rows
+    target = whole.clone()
+    with torch.no_grad():
+        zbpe.adjust_logits(target[:, 1:16], **g, out=target[:, 1:16])
+    assert torch.equal(target[:, 1:16], out) and not target[:, 0].any() and not target[:, 16].any()
 
 
 @gpu
