@@ -9,7 +9,9 @@ They run on libzbpe.so's kernels (include/zbpe.h states each one's definition), 
 stream, wait for nothing and can be captured into a HIP graph. Logits are float32, float16 or bfloat16 with any number of
 leading axes, ``[..., V]`` with V up to 65536; a per-row tensor has the leading axes' shape, and a plain number stands for
 all rows. Tensors of the wrong type, shape or device raise InvalidArgument before anything is launched. Results of a captured
-call are those of the eager one, bit for bit; no result depends on the order in which workgroups run.
+call are those of the eager one, bit for bit; no result depends on the order in which workgroups run. A backward pass is captured
+as any of torch's: warmed up on a side stream, and while no eager graph of the same leaves is alive (torch ties a leaf's gradient
+to the stream that first used it).
 """
 from __future__ import annotations
 
@@ -121,7 +123,7 @@ class _Rows:
 
     def on(self, t: torch.Tensor, name: str) -> None:
         _is_tensor(t, name)
-        if t.device != self.device:
+        if t.get_device() != self.index:
             raise InvalidArgument(f"{name} is on {t.device}, the logits are on {self.device}")
 
     def per_row(self, x, name: str, dtype: torch.dtype, keep: list) -> int:
