@@ -329,7 +329,7 @@ typedef struct zbpe_adjust {
     zbpe_rows logits;         /* F32, F16 or BF16 */
     zbpe_rows out;            /* the type of the logits, or F32; may be the logits themselves */
     zbpe_rows history;        /* I32 or I64; data NULL: none */
-    int64_t history_len;      /* tokens a row has room for */
+    int64_t history_len;      /* tokens a row has room for; all are read, those past its length count for nothing */
     const int32_t *lengths;         /* NULL: history_len; clamped to 0 .. history_len */
     const int32_t *prompt_lengths;  /* NULL: 0 */
     const float *repetition, *presence, *frequency; /* NULL: 1, 0, 0 */
