@@ -199,13 +199,13 @@ __device__ __forceinline__ int walk(const Automaton &g, int s, uint32_t at, uint
 //   - Of the others most end at their second byte.
 // Each wave queues what is left and walks it 64 at a time. The rows of the automaton that such walks need most, the state's own
 // and up to three that follow it (seven: 3 % slower, since every state pays for them), are in shared memory, their entries
-// replaced by the places of these rows (0 .. ROWS - 1; other states follow, -1: refused). The bits return to the order of ids in
-// shared memory. 2048 states x 65535 tokens in 193 us (a walk for each pair: 728), 600 x 32000 in 41; the 19 MB in and out would
+// replaced by the places of these rows (0 .. ROWS - 1, then REFUSED, then all other states). The bits return to the order of ids in
+// shared memory. 2048 states x 65535 tokens in 179 us (a walk for each pair: 728), 600 x 32000 in 38; the 19 MB in and out would
 // take 4. What bounds it: the instructions of classifying and walking, then the latency of a state's rows.
 template <int NT>
 __global__ __launch_bounds__(NT) void grammar_masks_kernel(Automaton g, const int32_t *states, int64_t rows, uint32_t *masks, int slices, int per) {
-    constexpr int ROWS = 4, SLICES = ZBPE_MAX_VOCAB / INDEX_SLICE, SLICE_WORDS = INDEX_SLICE / 32;
-    __shared__ int next[ROWS][256];
+    constexpr int ROWS = 4, REFUSED = ROWS, SLICES = ZBPE_MAX_VOCAB / INDEX_SLICE, SLICE_WORDS = INDEX_SLICE / 32;
+    __shared__ int next[ROWS + 1][256];  // the last row: once refused, always refused
     __shared__ int place[ROWS];  // the states of these rows
     __shared__ uint32_t live[8], turns[2][4];  // the bytes that the state takes; the classes with a byte that changes it
     __shared__ uint32_t bits[SLICES * SLICE_WORDS];
@@ -273,12 +273,12 @@ __global__ __launch_bounds__(NT) void grammar_masks_kernel(Automaton g, const in
             }
         }
         __syncthreads();
-        for (int i = t; i < ROWS * 256; i += NT) {
-            const int s = place[i >> 8];
+        for (int i = t; i < (ROWS + 1) * 256; i += NT) {
+            const int s = i < ROWS * 256 ? place[i >> 8] : -1;
             int to = i < 256 ? next[0][i] : s >= 0 && known ? g.next[(int64_t)s * 256 + (i & 255)] : -1;
-            if (!inside(g, to)) to = -1;
+            if (!inside(g, to)) to = REFUSED;
             else {
-                int at = to + ROWS;
+                int at = to + ROWS + 1;
 #pragma unroll
                 for (int k = ROWS - 1; k >= 0; k--)
                     if (to == place[k]) at = k;
@@ -299,19 +299,20 @@ __global__ __launch_bounds__(NT) void grammar_masks_kernel(Automaton g, const in
             int s = 0;
 #pragma unroll
             for (int j = 0; j < INDEX_BYTES; j++) {
-                const bool on = s >= 0 && j < length;
-                if (!__any(on)) break;
+                if (j % 3 == 0 && !__any(s != REFUSED && j < length)) break;
                 const int b = j < INDEX_HEAD ? x.byte(j) : y.byte(j - INDEX_HEAD);
-                if (on) {
-                    if (s < ROWS) s = next[s][b];
-                    else {
-                        s = g.next[(int64_t)(s - ROWS) * 256 + b];
-                        s = inside(g, s) ? s == s0 ? 0 : s + ROWS : -1;
-                    }
+                int to = next[min(s, REFUSED)][b];
+                if (s > REFUSED && j < length) {
+                    to = g.next[(int64_t)(s - ROWS - 1) * 256 + b];
+                    to = inside(g, to) ? to == s0 ? 0 : to + ROWS + 1 : REFUSED;
                 }
+                s = j < length ? to : s;
             }
-            if (length > INDEX_BYTES && s >= 0) s = walk(g, s < ROWS ? place[s] : s - ROWS, g.offsets[id] + INDEX_BYTES, g.offsets[id + 1]);
-            if (s >= 0) allow(id);
+            if (length > INDEX_BYTES && s != REFUSED) {
+                s = walk(g, s < ROWS ? place[s] : s - ROWS - 1, g.offsets[id] + INDEX_BYTES, g.offsets[id + 1]);
+                if (s < 0) s = REFUSED;
+            }
+            if (s != REFUSED) allow(id);
         };
 
         const int n = listed;
@@ -328,10 +329,10 @@ __global__ __launch_bounds__(NT) void grammar_masks_kernel(Automaton g, const in
                 on = !((x.classes[0] & turns_low) | (x.classes[1] & turns_high));
                 if (!on) {
                     const int s = next[0][x.byte(0)];
-                    if (s >= 0) {
+                    if (s != REFUSED) {
                         if (length == 1) on = true;
-                        else if (s >= ROWS) open = true;
-                        else if (next[s][x.byte(1)] >= 0) {
+                        else if (s > REFUSED) open = true;
+                        else if (next[s][x.byte(1)] != REFUSED) {
                             on = length == 2;
                             open = !on;
                         }
