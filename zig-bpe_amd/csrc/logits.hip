@@ -200,7 +200,7 @@ __device__ __forceinline__ int walk(const Automaton &g, int s, uint32_t at, uint
 // Each wave queues what is left and walks it 64 at a time. The rows of the automaton that such walks need most, the state's own
 // and up to three that follow it (seven: 3 % slower, since every state pays for them), are in shared memory, their entries
 // replaced by the places of these rows (0 .. ROWS - 1, then REFUSED, then all other states). The bits return to the order of ids in
-// shared memory. 2048 states x 65535 tokens in 179 us (a walk for each pair: 728), 600 x 32000 in 38; the 19 MB in and out would
+// shared memory. 2048 states x 65535 tokens in 168 us (a walk for each pair: 728), 600 x 32000 in 37; the 19 MB in and out would
 // take 4. What bounds it: the instructions of classifying and walking, then the latency of a state's rows.
 template <int NT>
 __global__ __launch_bounds__(NT) void grammar_masks_kernel(Automaton g, const int32_t *states, int64_t rows, uint32_t *masks, int slices, int per) {
@@ -212,7 +212,7 @@ __global__ __launch_bounds__(NT) void grammar_masks_kernel(Automaton g, const in
     __shared__ uint16_t list[SLICES * INDEX_SLICE / 64];
     __shared__ uint16_t queues[NT / 64][128];
     __shared__ int listed;
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, words = (g.vocab + 31) / 32;
+    const int t = threadIdx.x, lane = t & 63, wave = (int)uniform((uint32_t)t >> 6), words = (g.vocab + 31) / 32;
     const int parts = (slices + per - 1) / per;
     const IndexView index(g.index, g.vocab);
     uint16_t *queue = queues[wave];
@@ -315,33 +315,28 @@ __global__ __launch_bounds__(NT) void grammar_masks_kernel(Automaton g, const in
             if (s != REFUSED) allow(id);
         };
 
-        const int n = listed;
-        int queued = 0, at = 0;
+        const int n = (int)uniform((uint32_t)listed);
+        auto group = [&](int i) { return (int)uniform((uint32_t)list[i]) * 64; };
+        int queued = 0, first = 0;
         IndexHead ahead{};
-        if (wave < n) ahead = index.heads[at = list[wave] * 64 + lane];
+        if (wave < n) ahead = index.heads[(first = group(wave)) + lane];
         for (int i = wave; i < n; i += NT / 64) {
             const IndexHead x = ahead;
-            const int here = at;
-            if (i + NT / 64 < n) ahead = index.heads[at = list[i + NT / 64] * 64 + lane];
-            const int id = here / INDEX_SLICE * INDEX_SLICE + x.id(), length = x.length();
-            bool on = false, open = false;
-            if (length && id != g.end) {
-                on = !((x.classes[0] & turns_low) | (x.classes[1] & turns_high));
-                if (!on) {
-                    const int s = next[0][x.byte(0)];
-                    if (s != REFUSED) {
-                        if (length == 1) on = true;
-                        else if (s > REFUSED) open = true;
-                        else if (next[s][x.byte(1)] != REFUSED) {
-                            on = length == 2;
-                            open = !on;
-                        }
-                    }
-                }
+            const int from = first;
+            if (i + NT / 64 < n) ahead = index.heads[(first = group(i + NT / 64)) + lane];
+            const int id = from / INDEX_SLICE * INDEX_SLICE + x.id(), length = x.length();
+            const bool asked = length && id != g.end;
+            bool on = asked && !((x.classes[0] & turns_low) | (x.classes[1] & turns_high)), open = false;
+            if (__any(asked && !on)) {
+                const int s = next[0][x.byte(0)];
+                const bool fits = length == 1 ? s != REFUSED : s > REFUSED || next[min(s, REFUSED)][x.byte(1)] != REFUSED;
+                const bool ends = length == 1 || (length == 2 && s < REFUSED);
+                open = asked && !on && fits && !ends;
+                on = on || (asked && fits && ends);
             }
             if (on) allow(id);
             const uint64_t b = __ballot(open);
-            if (open) queue[queued + __popcll(b & ((1ull << lane) - 1))] = (uint16_t)here;
+            if (open) queue[queued + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)b, 0))] = (uint16_t)(from + lane);
             queued += __popcll(b);
             if (queued >= 64) {
                 __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
