@@ -35,6 +35,7 @@ _GRAMMAR = struct.Struct("@PPiiPPiP")
 _ADJUST = struct.Struct("@Iiqq" + 3 * _ROWS + "qPPPPPPPPiiPqP")
 _DRAW = struct.Struct("@Iiqq" + _ROWS + "PPPPPPP")
 _LOGPROBS = struct.Struct("@Iiqq" + _ROWS + "PiPPP")
+_MATRIX = struct.Struct("@" + _ROWS)
 _NO_ROWS = (0, 0, 0, 0)
 
 _checked = None
@@ -413,10 +414,10 @@ class _Adjust(torch.autograd.Function):
         d_values = torch.empty_like(x.bias_values, memory_format=torch.contiguous_format) if wants[2] else None
         L = _library()
         space = L.zbpe_adjust_workspace(at.rows, at.cols) if wants[1] else 0
-        workspace = torch.empty(space, dtype=torch.uint8, device=at.device)
-        rows = None if d_logits is None else struct.pack("@" + _ROWS, *at.matrix(d_logits, keep))
+        workspace = torch.empty(space, dtype=torch.uint8, device=at.device) if space else None
+        rows = None if d_logits is None else _MATRIX.pack(*at.matrix(d_logits, keep))
         _check(L.zbpe_adjust_logits_grad(at.device.index, _stream(at.device), args, rows, 0 if d_bias is None else d_bias.data_ptr(),
-                                         0 if d_values is None else d_values.data_ptr(), workspace.data_ptr(), space))
+                                         0 if d_values is None else d_values.data_ptr(), 0 if workspace is None else workspace.data_ptr(), space))
         return d_logits, d_bias, d_values, None, None
 
 
@@ -518,7 +519,7 @@ class _Logprobs(torch.autograd.Function):
         grad = grad.contiguous()
         d_logits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         _check(_library().zbpe_token_logprobs_grad(at.device.index, _stream(at.device), args, grad.data_ptr(),
-                                                   struct.pack("@" + _ROWS, *at.matrix(d_logits, keep))))
+                                                   _MATRIX.pack(*at.matrix(d_logits, keep))))
         return d_logits, None, None
 
 
@@ -526,7 +527,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, temperature=No
     """float32 [...]: the log-probability of each row's token (int32 or int64 [...]) under softmax(logits / temperature), with
     the gradient with respect to the logits. Negative tokens (padding) are not scored: 0, and no gradient. A token past the
     last column gives NaN; so does +inf or NaN among the logits. A row of -inf alone gives -inf, and no gradient."""
-    _Rows(logits)
+    _is_tensor(logits, "logits")
     if torch.is_grad_enabled():
         _no_gradient(temperature=temperature)
     if torch.is_grad_enabled() and logits.requires_grad:
