@@ -371,8 +371,8 @@ __global__ __launch_bounds__(256) void grammar_advance_kernel(Automaton g, const
 // A workgroup takes a slice of columns over a run of rows, 32 bytes of logits a thread. What a row needs from memory is on its
 // way while the row before it is worked on. The row's history is counted in shared memory: a bit for each column that is in it
 // (the bits of one load's columns in one byte, which is 0 for most loads) and how often behind the prompt. Whoever uses a bit
-// or a count clears it. Bound by memory: 4096 rows of 32000 bf16, 500 tokens of history each, in 143 us (0.52 GB, 3.7 TB/s; a copy
-// reaches 4.9), the gradient in 167.
+// or a count clears it. Bound by memory: 4096 rows of 32000 bf16, up to 500 tokens of history each, in 146 us (0.52 GB, 3.6 TB/s; a
+// copy reaches 4.9), the gradient in 173.
 constexpr int ADJUST_THREADS = 512, ADJUST_PACKS = 2, ADJUST_RUN = 32;
 constexpr int ADJUST_GROUPS = 2;  // on a CU at a time: 4 waves on a SIMD leave 128 registers to a thread
 template <class T>
@@ -1268,8 +1268,9 @@ __device__ __forceinline__ int64_t token_of(const Logprobs &a, int64_t r) {
     return a.wide_ids ? ((const int64_t *)a.tokens)[r] : (int64_t)((const int32_t *)a.tokens)[r];
 }
 
-// One pass with a running maximum and sum. TPR threads go over one row, AHEAD loads of 16 bytes each at a time (one at a time:
-// 151 us instead of 110 for 8192 rows of 32000 bf16, 4.8 TB/s). Short rows take a wave each. Bound by memory.
+// One pass with a running maximum and sum. TPR threads go over one row, AHEAD loads of 16 bytes each at a time. 8192 rows of 32000
+// bf16 in 122 us (0.52 GB, 4.3 TB/s; with one load at a time the kernel took 1.37 times as long). Short rows take a wave each. Bound
+// by memory.
 template <class T, int TPR>
 __global__ __launch_bounds__(256) void logprobs_kernel(Logprobs a) {
     constexpr int N = Pack<T>::N, PER = 256 / TPR, AHEAD = 4;
@@ -1340,7 +1341,7 @@ __global__ __launch_bounds__(256) void logprobs_kernel(Logprobs a) {
     }
 }
 
-// One slice of columns (blockIdx.y) of one row after another. 8192 rows of 32000 bf16 in 190 us (1.05 GB read and written, 5.5 TB/s
+// One slice of columns (blockIdx.y) of one row after another. 8192 rows of 32000 bf16 in 188 us (1.05 GB read and written, 5.6 TB/s
 // with what the caches keep of the forward pass; the loads come before the scalars that they do not need). Bound by memory.
 template <class T>
 __global__ __launch_bounds__(256) void logprobs_grad_kernel(Logprobs a) {
