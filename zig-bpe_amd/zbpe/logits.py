@@ -80,6 +80,11 @@ def _no_gradient(**named) -> None:
             raise InvalidArgument(f"{name} has no gradient here: detach it")
 
 
+def _written(out: torch.Tensor) -> None:
+    """A caller's tensor was written by its pointer: torch is told, so that a backward pass that needs what stood there raises."""
+    torch.autograd.graph.increment_version(out)
+
+
 class _Rows:
     """How the rows of one call are numbered: by the logits' leading axes, in two levels."""
 
@@ -276,6 +281,7 @@ class Grammar:
             states = self._vector(states, "states")
         lead = (self.states,) if states is None else states.shape
         shape = (*lead, self.vocabulary.words)
+        written = out is not None
         if out is None:
             out = torch.empty(shape, dtype=torch.int32, device=device)
         else:
@@ -285,6 +291,8 @@ class Grammar:
         rows = self.states if states is None else states.numel()
         _check(_library().zbpe_grammar_masks(device.index, _stream(device), self._packed(),
                                              None if states is None else states.data_ptr(), rows, out.data_ptr()))
+        if written:
+            _written(out)
         return out
 
     def advance(self, states: torch.Tensor, tokens: torch.Tensor) -> torch.Tensor:
@@ -447,12 +455,14 @@ def adjust_logits(logits: torch.Tensor, *, history: Optional[torch.Tensor] = Non
     if torch.is_grad_enabled():
         _no_gradient(repetition=repetition, presence=presence, frequency=frequency)
     if out is not None:
-        _need(not learns, "out goes without gradients")
         _is_tensor(out, "out")
+        _need(not learns and not (out.requires_grad and torch.is_grad_enabled()), "out goes without gradients")
         if not (out.shape == logits.shape and out.device == logits.device and out.dtype in (logits.dtype, torch.float32)):
             raise InvalidArgument(f"out is not {logits.dtype} or float32 of shape {tuple(logits.shape)} on {logits.device}")
         _need(_Rows(logits).matrix(out, [])[0] == out.data_ptr(), "out has strides that its rows cannot be written by")
-        return _adjust(logits, out, x)
+        _adjust(logits, out, x)
+        _written(out)
+        return out
     if learns:
         return _Adjust.apply(logits, bias, bias_values, x, logits.dtype)
     return _adjust(logits, torch.empty(logits.shape, dtype=logits.dtype, device=logits.device), x)
