@@ -79,3 +79,36 @@ def test_out_without_anything_saved():
     before = z._version
     zbpe.adjust_logits(z, **g)  # (what is only read keeps its version)
     assert z._version == before
+
+
+# ---- forward-mode derivatives --------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_forward_mode_is_refused(device):
+    """a tangent that no operator here carries is not dropped: the call raises, whatever requires_grad and no_grad say"""
+    z, x = adjust_case(4, 300, 1)
+    z, x = z.to(device), {k: v.to(device) for k, v in x.items()}
+    t = torch.ones(4, device=device)
+    tokens = torch.zeros(4, dtype=torch.int64, device=device)
+    with forward_ad.dual_level():
+        dual = lambda a: forward_ad.make_dual(a, torch.ones_like(a))  # noqa: E731
+        calls = [lambda: zbpe.adjust_logits(dual(z), **x), lambda: zbpe.adjust_logits(dual(z)[:, 1:], bias=x["bias"][1:]),
+                 lambda: zbpe.token_logprobs(dual(z), tokens), lambda: zbpe.token_logprobs(z, tokens, temperature=dual(t)),
+                 lambda: zbpe.adjust_logits(dual(z), out=torch.empty_like(z)), lambda: zbpe.adjust_logits(z, out=dual(torch.empty_like(z)))]
+        for name in ("bias", "bias_values", "repetition", "presence", "frequency"):
+            calls.append(lambda name=name: zbpe.adjust_logits(z, **{**x, name: dual(x[name])}))
+        for call in calls:
+            with pytest.raises(zbpe.InvalidArgument, match="tangent"):
+                call()
+            with torch.no_grad(), pytest.raises(zbpe.InvalidArgument, match="tangent"):
+                call()
+        if device == "cpu":
+            return
+        # nothing is dropped where nothing is differentiated: inference mode, logits that are cut off, the draw
+        want = zbpe.token_logprobs(z, tokens)
+        assert torch.equal(zbpe.token_logprobs(dual(z).detach(), tokens), want)
+        d = dual(z)
+        with torch.inference_mode():
+            assert torch.equal(zbpe.token_logprobs(d, tokens), want)
+        zbpe.draw_tokens(dual(z), torch.zeros(4, device=device))

@@ -21,6 +21,7 @@ from typing import NamedTuple, Optional
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from . import _STATUS, InternalError, InvalidArgument, Merges, ZbpeError, _ptr, load_library, vocabStart
 
@@ -78,6 +79,16 @@ def _no_gradient(**named) -> None:
     for name, x in named.items():
         if isinstance(x, torch.Tensor) and x.requires_grad:
             raise InvalidArgument(f"{name} has no gradient here: detach it")
+
+
+def _no_tangent(**named) -> None:
+    """No operator here has a forward-mode derivative. (A tensor with a tangent does not require a gradient, so that torch's own
+    refusal is not reached; and no_grad does not switch tangents off.)"""
+    if forward_ad._current_level < 0 or not torch._C._is_fwd_grad_enabled():  # (the usual case: no tensor has one)
+        return
+    for name, x in named.items():
+        if isinstance(x, torch.Tensor) and forward_ad.unpack_dual(x).tangent is not None:
+            raise InvalidArgument(f"{name} has a tangent, and there is no forward-mode derivative here: detach it")
 
 
 def _written(out: torch.Tensor) -> None:
@@ -447,13 +458,14 @@ def adjust_logits(logits: torch.Tensor, *, history: Optional[torch.Tensor] = Non
     history: int32 or int64 [..., n]; lengths and prompt_lengths (int32 [...]): how many of a row's tokens count, and how
     many of these are the prompt's. History and bias tokens outside 0 .. V - 1 are passed over.
 
-    Gradients go to logits, bias and bias_values. out: where to write (the logits' type or float32; it may be the logits
+    Gradients go to logits, bias and bias_values; tangents (forward mode) are refused. out: where to write (the logits' type or float32; it may be the logits
     themselves), without gradients."""
     x = _Terms(history, lengths, prompt_lengths, repetition, presence, frequency, bias, bias_tokens, bias_values, masks, states)
     _is_tensor(logits, "logits")
     learns = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (logits, bias, bias_values))
     if torch.is_grad_enabled():
         _no_gradient(repetition=repetition, presence=presence, frequency=frequency)
+    _no_tangent(logits=logits, bias=bias, bias_values=bias_values, repetition=repetition, presence=presence, frequency=frequency, out=out)
     if out is not None:
         _is_tensor(out, "out")
         _need(not learns and not (out.requires_grad and torch.is_grad_enabled()), "out goes without gradients")
@@ -478,7 +490,8 @@ def draw_tokens(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature=Non
     less: all), top_p of these the first whose predecessors hold less than this share of their sum, min_p of these the
     ones with at least this share of the largest weight. The token is the first, by id, at which the sum of the kept
     weights exceeds uniforms (float32 [...], in [0, 1)) times the whole. A temperature of 0 or less takes the largest
-    logit. A row without a logit above -inf gives token -1; NaN counts as -inf."""
+    logit. A row without a logit above -inf gives token -1; NaN counts as -inf. Neither result has a gradient: token_logprobs
+    scores drawn tokens with one."""
     at, keep = _Rows(logits), []
     logits = logits.detach()
     _is_tensor(uniforms, "uniforms")
@@ -535,11 +548,12 @@ class _Logprobs(torch.autograd.Function):
 
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, temperature=None) -> torch.Tensor:
     """float32 [...]: the log-probability of each row's token (int32 or int64 [...]) under softmax(logits / temperature), with
-    the gradient with respect to the logits. Negative tokens (padding) are not scored: 0, and no gradient. A token past the
+    the gradient with respect to the logits (tangents are refused). Negative tokens (padding) are not scored: 0, and no gradient. A token past the
     last column gives NaN; so does +inf or NaN among the logits. A row of -inf alone gives -inf, and no gradient."""
     _is_tensor(logits, "logits")
     if torch.is_grad_enabled():
         _no_gradient(temperature=temperature)
+    _no_tangent(logits=logits, temperature=temperature)
     if torch.is_grad_enabled() and logits.requires_grad:
         return _Logprobs.apply(logits, tokens, temperature)
     return _logprobs(logits.detach(), tokens, temperature, None)
