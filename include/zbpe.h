@@ -261,7 +261,9 @@ zbpe_status zbpe_zig_order_winner(const uint32_t *first_pos, const uint32_t *key
  * Operators over device buffers of the caller, on the caller's device and stream (a hipStream_t; NULL: the default stream).
  * They take no context, allocate nothing, wait for nothing (they may be captured into a HIP graph) and may be called from
  * several threads. On failure zbpe_last_error(NULL) is the calling thread's message. A call whose arguments are refused
- * launches nothing. Tokens are the ids that zbpe_train makes, so a vocabulary has at most ZBPE_MAX_VOCAB of them.
+ * launches nothing. What a call writes overlaps nothing that it reads, nor anything else that it writes, unless an argument says
+ * so below; overlapping logits, gradients of logits, masks and states are refused. Tokens are the ids that zbpe_train makes, so
+ * a vocabulary has at most ZBPE_MAX_VOCAB of them.
  *
  * Rows: a matrix of logits has `rows` rows of `cols` elements that lie side by side; row r starts
  * (r / inner) * outer_stride + (r % inner) * inner_stride elements behind `data` (so [batch, time, cols] views with a cut
@@ -327,7 +329,8 @@ typedef struct zbpe_adjust {
     int32_t cols;             /* 1 .. ZBPE_MAX_VOCAB */
     int64_t rows, inner;      /* inner >= 1 */
     zbpe_rows logits;         /* F32, F16 or BF16 */
-    zbpe_rows out;            /* the type of the logits, or F32; may be the logits themselves */
+    zbpe_rows out;            /* the type of the logits, or F32; may be the logits themselves (the same
+                                 address, strides and type), and overlaps them in no other way */
     zbpe_rows history;        /* I32 or I64; data NULL: none */
     int64_t history_len;      /* tokens a row has room for; all are read, those past its length count for nothing */
     const int32_t *lengths;         /* NULL: history_len; clamped to 0 .. history_len */
@@ -347,7 +350,7 @@ typedef struct zbpe_adjust {
 zbpe_status zbpe_adjust_logits(int device, void *stream, const zbpe_adjust *args);
 
 /* Its gradient: `args` as in the call, args->out the gradient of its output (only read), args->logits the same logits. Writes
- * grad_logits (the logits' type, rows of its own), grad_bias [cols] and grad_bias_values [rows][n_biases]; each may be NULL.
+ * grad_logits (the logits' type; memory of its own), grad_bias [cols] and grad_bias_values [rows][n_biases]; each may be NULL.
  * A masked element passes no gradient. grad_bias needs a workspace of zbpe_adjust_workspace(rows, cols) bytes, which no
  * other call uses until this one is done; it sums rows in an order that depends on rows, cols and the type alone. */
 size_t zbpe_adjust_workspace(int64_t rows, int32_t cols);
@@ -384,7 +387,8 @@ zbpe_status zbpe_draw_tokens(int device, void *stream, const zbpe_draw *args);
  * token is not scored: 0, and no gradient. A token past the last column gives NaN. A row without anything above -inf gives
  * -inf and no gradient. stats ([rows][2] f32: the row's maximum, and the sum of exp(z - its maximum)) is what the gradient
  * needs; it may be NULL when none follows. temperature: NULL: 1; positive.
- * zbpe_token_logprobs_grad writes grad_logits (the logits' type) = grad[r] / temperature[r] * ([v == t] - softmax(z)[v]). */
+ * zbpe_token_logprobs_grad writes grad_logits (the logits' type; may be the logits themselves, as `out` above)
+ * = grad[r] / temperature[r] * ([v == t] - softmax(z)[v]). */
 typedef struct zbpe_logprobs {
     uint32_t struct_size;     /* sizeof(zbpe_logprobs) */
     int32_t cols;

@@ -112,3 +112,165 @@ def test_forward_mode_is_refused(device):
         with torch.inference_mode():
             assert torch.equal(zbpe.token_logprobs(d, tokens), want)
         zbpe.draw_tokens(dual(z), torch.zeros(4, device=device))
+
+
+# ---- memory that overlaps ------------------------------------------------------------------------------------------------------
+
+
+def bytes_of(data, outer, inner, rows, per, cols, element):
+    """the addresses of a matrix's elements, by zbpe_rows' rule"""
+    r = np.arange(rows)
+    starts = data + ((r // per) * outer + (r % per) * inner) * element
+    return set((starts[:, None] + np.arange(cols * element)).reshape(-1).tolist()) if rows else set()
+
+
+def test_memory_that_is_written_against_all_that_is_read():
+    """Matrices and arrays at random places of a small memory: a gradient that shares a byte with anything that the call reads is
+    refused for that, any other one reaches the check behind it (of the workspace, which is missing here: nothing is launched)."""
+    from zbpe import logits as ops
+
+    L, rng = ops._library(), np.random.default_rng(0)
+    seen = {True: 0, False: 0}
+    for _ in range(6000):
+        rows, per, cols = int(rng.integers(1, 9)), int(rng.integers(1, 5)), int(rng.integers(1, 12))
+        kind = int(rng.integers(0, 3))
+        element = 4 if kind == 0 else 2
+        inside = lambda: int(rng.integers(0, 500) // 8 * 8) + 4096  # noqa: E731
+
+        def matrix(n, size, apart):
+            inner = int(rng.choice([n, n + rng.integers(0, 20), 2 * n, 0 if not apart else n]))
+            outer = int(rng.choice([inner * per, max(inner * (per - 1) + n, 0) + rng.integers(0, 20)]))
+            if rng.random() < 0.3:  # rows of different outer steps between each other
+                outer, inner = int(n + rng.integers(0, 6)), int((n + 6) * ((rows + per - 1) // per) + rng.integers(0, 6))
+            if rng.random() < 0.1:
+                return inside() + 600, -outer, -inner
+            return inside(), outer, inner
+
+        if rng.random() < 0.5:  # the same strides for all, at different places
+            strides = matrix(cols, element, True)[1:]
+            places = [(inside(), *strides) for _ in range(3)]
+        else:
+            places = [matrix(cols, element, i == 0) for i in range(3)]
+        wide_up = rng.random() < 0.3
+        hist = matrix(5, 4, False) if rng.random() < 0.5 else None
+        arrays = {}
+        for name, n in (("lengths", 4 * rows), ("prompt", 4 * rows), ("theta", 4 * rows), ("presence", 4 * rows), ("frequency", 4 * rows),
+                        ("bias", 4 * cols), ("tokens", 8 * rows), ("values", 8 * rows), ("masks", 4 * 6), ("states", 4 * rows)):
+            if rng.random() < 0.15:
+                arrays[name] = (inside(), n)
+        if ("tokens" in arrays) != ("values" in arrays):
+            arrays.pop("tokens", None), arrays.pop("values", None)
+        if "masks" not in arrays:
+            arrays.pop("states", None)
+        elif "states" not in arrays:
+            arrays.pop("masks")
+        place = lambda name: arrays.get(name, (0, 0))[0]  # noqa: E731
+        (gp, go, gi), (zp, zo, zi), (up, uo, ui) = places
+        args = ops._ADJUST.pack(
+            ops._ADJUST.size, cols, rows, per, zp, zo, zi, kind, up, uo, ui, 0 if wide_up else kind,
+            *((hist[0], hist[1], hist[2], 3) if hist else (0, 0, 0, 0)), 5 if hist else 0, place("lengths"), place("prompt"), place("theta"),
+            place("presence"), place("frequency"), place("bias"), place("tokens"), place("values"), 2 if "tokens" in arrays else 0, 1,
+            place("masks"), 6 if "masks" in arrays else 0, place("states"))
+        status = L.zbpe_adjust_logits_grad(0, None, args, ops._MATRIX.pack(gp, go, gi, kind), 64, 0, 64, 0)
+        message = L.zbpe_last_error(None).decode()
+        assert status == 5
+        if "the rows of grad_logits overlap" in message:
+            continue
+        read = bytes_of(zp, zo, zi, rows, per, cols, element) | bytes_of(up, uo, ui, rows, per, cols, 4 if wide_up else element)
+        if hist:
+            read |= bytes_of(*hist, rows, per, 5, 4)
+        for at, n in arrays.values():
+            read |= set(range(at, at + n))
+        overlap = bool(bytes_of(gp, go, gi, rows, per, cols, element) & read)
+        assert ("grad_logits overlaps" in message) == overlap and ("workspace of 0 bytes" in message) != overlap, (message, args)
+        seen[overlap] += 1
+    assert min(seen.values()) > 500
+
+
+def test_masks_and_states_that_overlap_what_is_read():
+    from zbpe import logits as ops
+
+    L = ops._library()
+    grammar = ops._GRAMMAR.pack(1 << 20, 1 << 21, 300, -1, 1 << 22, 1 << 23, 5, 1 << 24)  # (words: 10)
+    for states, out, words in ((4096, 4096, "states"), (4096 + 196, 4096, "states"), (4096, 4096 + 8, "states"),
+                               (4096, (1 << 22) + 5000, "automaton"), (4096, (1 << 22) - 196, "automaton"), (4096, (1 << 23) - 8, "automaton"),
+                               (4096, (1 << 24) + 300 * 32, "index")):
+        assert L.zbpe_grammar_masks(0, None, grammar, states, 5, out) == 5
+        assert "masks overlaps" in L.zbpe_last_error(None).decode() and words in L.zbpe_last_error(None).decode()
+    for states, tokens, out, words in ((4096, 8192, 4100, "states"), (4096, 8192, 8188, "tokens"), (4096, 8192, 1 << 22, "automaton")):
+        assert L.zbpe_grammar_advance(0, None, grammar, states, tokens, 5, out) == 5
+        assert "out overlaps" in L.zbpe_last_error(None).decode() and words in L.zbpe_last_error(None).decode()
+
+
+def test_out_that_overlaps_in_part():
+    """the forward call, and the scores' gradient, by the same rule"""
+    from zbpe import logits as ops
+
+    L = ops._library()
+    none = (0, 0, 0, 0)
+
+    def adjust(z, out, rows=4, inner=4, history=none, n=0, bias=0):
+        return L.zbpe_adjust_logits(0, None, ops._ADJUST.pack(ops._ADJUST.size, 300, rows, inner, *z, *out, *history, n, 0, 0, 0, 0, 0, bias, 0, 0, 0, 0, 0, 0, 0))
+
+    base = 1 << 20
+    for z, out, kw, words in (((base, 0, 300, 0), (base + 4, 0, 300, 0), {}, "the logits"),         # one column on
+                              ((base, 0, 300, 0), (base + 1200, 0, 300, 0), {}, "the logits"),      # one row on
+                              ((base, 0, 300, 1), (base, 0, 300, 0), {}, "the logits"),             # 32 bits over 16
+                              ((base, 0, 600, 0), (base + 1196, 0, 600, 0), {}, "the logits"),      # beside each other but for one
+                              ((base, 0, 300, 0), (base, 0, 301, 0), {}, "the logits"),             # other strides
+                              ((base, 0, 0, 0), (base - 1200, 0, 300, 0), {}, "the logits"),        # a broadcast row among them
+                              ((base, 0, 300, 0), (2 * base, 0, 300, 0), {"history": (2 * base + 4796, 0, 50, 3), "n": 50}, "history"),
+                              ((base, 0, 300, 0), (2 * base, 0, 300, 0), {"bias": 2 * base - 1196}, "bias"),
+                              ((base, 0, 300, 0), (base, 0, 300, 0), {"bias": base + 2400}, "bias")):
+        assert adjust(z, out, **kw) == 5
+        assert f"out overlaps {words}" in L.zbpe_last_error(None).decode()
+    for grad, words in ((base + 4, "the logits"), (2 * base - 8, "the tokens"), (3 * base, "grad"), (4 * base + 24, "stats")):
+        args = ops._LOGPROBS.pack(ops._LOGPROBS.size, 300, 4, 4, base, 0, 300, 0, 2 * base, 3, 0, 0, 4 * base)
+        assert L.zbpe_token_logprobs_grad(0, None, args, 3 * base, ops._MATRIX.pack(grad, 0, 300, 0)) == 5
+        assert f"grad_logits overlaps {words}" in L.zbpe_last_error(None).decode()
+
+
+@gpu
+@pytest.mark.parametrize("kind", [torch.float32, torch.bfloat16])
+def test_out_beside_the_logits(kind):
+    """what shares a buffer and no element is written as before: halves of rows, alternate rows, another dtype's rows in between;
+    what shares some is refused and not touched"""
+    z, x = adjust_case(12, 700, 4, kind=kind)
+    g = to_gpu(x)
+    want = zbpe.adjust_logits(z.cuda(), **g)
+    wide = torch.full((12, 1500), 7.0, dtype=kind, device="cuda")
+    halves = wide[:, 3:703], wide[:, 703:1403]
+    rows = wide.view(24, 750)[:, 1:701]
+    for source, out in (halves, halves[::-1], (rows[::2], rows[1::2])):
+        wide.fill_(7.0)
+        source.copy_(z)
+        assert zbpe.adjust_logits(source, **g, out=out) is out
+        assert torch.equal(out, want) and torch.equal(source, z.cuda())
+        assert int((wide == 7).sum()) >= 12 * 100
+    three = wide[:, 3:703].view(3, 4, 700)
+    three.copy_(z.view(3, 4, 700))
+    shaped = {k: v.view(3, 4, *v.shape[1:]) if k not in ("bias", "masks") else v for k, v in g.items()}
+    assert torch.equal(zbpe.adjust_logits(three, **shaped, out=three).reshape(12, 700), want)  # in place, by another view
+    row = wide[5:6, :700]
+    row.copy_(z[:1])
+    spread = torch.cat([wide[:5], wide[6:], wide[:1]])[:, :700]
+    assert zbpe.adjust_logits(row.expand(12, -1), **g, out=spread) is spread
+    buffer = torch.arange(13 * 700, device="cuda").view(13, 700).to(kind)
+    was = buffer.clone()
+    for source, out in ((buffer[:12], buffer[1:]), (buffer[1:], buffer[:12]), (buffer[:12, :-1], buffer[:12, 1:]),
+                        (buffer[1:2].expand(12, -1), buffer[:12])):
+        terms = {"presence": 1.0, "history": g["history"]}
+        with pytest.raises(zbpe.InvalidArgument, match="out overlaps the logits"):
+            zbpe.adjust_logits(source, **terms, out=out)
+    bias = torch.zeros(12 * 700, device="cuda")
+    with pytest.raises(zbpe.InvalidArgument, match="out overlaps bias"):
+        zbpe.adjust_logits(z.float().cuda(), bias=bias[700:1400], out=bias.view(12, 700))
+    masks = torch.zeros(13, 22, dtype=torch.int32, device="cuda")
+    with pytest.raises(zbpe.InvalidArgument, match="out overlaps masks"):
+        zbpe.adjust_logits(torch.zeros(1, 20, device="cuda"), masks=masks[:1], out=masks[:1, 1:21].view(torch.float32))
+    grammar = zbpe.Grammar(zbpe.Vocabulary([], 300), torch.zeros(13 * 10, 256, dtype=torch.int32))
+    states = torch.zeros(130, dtype=torch.int32, device="cuda")
+    with pytest.raises(zbpe.InvalidArgument, match="masks overlaps states"):
+        grammar.masks(states[:13], out=states.view(13, 10))
+    torch.cuda.synchronize()
+    assert torch.equal(buffer, was) and not bias.any() and not masks.any() and not states.any()

@@ -7,6 +7,7 @@
 
 #include <exception>
 #include <new>
+#include <utility>
 
 #include "../../include/zbpe.h"
 #include "logits.hpp"
@@ -1428,6 +1429,120 @@ static zbpe_status check_written(const char *what, const char *name, const zbpe_
     return ok ? ZBPE_OK : refuse(ZBPE_INVALID_ARGUMENT, "%s: the rows of %s overlap", what, name);
 }
 
+// The memory of a matrix or an array: n[0] * n[1] pieces of `size` bytes, step[0] and step[1] bytes apart, step[0] >= step[1].
+using wide = __int128;
+struct Pieces {
+    wide from = 0, size = 0, step[2] = {1, 1}, n[2] = {0, 0};  // no pieces
+
+    static Pieces array(const void *data, wide bytes) {
+        Pieces p;
+        if (!data || bytes <= 0) return p;
+        p.from = (wide)(uintptr_t)data;
+        p.size = bytes;
+        p.n[0] = p.n[1] = 1;
+        return p;
+    }
+    static Pieces rows(const void *data, wide bytes, int64_t n_outer, wide outer_step, int64_t n_inner, wide inner_step) {
+        Pieces p = array(data, bytes);
+        if (!p.size || n_outer < 1 || n_inner < 1) return Pieces();
+        const int64_t n[2] = {n_outer, n_inner};
+        const wide steps[2] = {outer_step, inner_step};
+        for (int i = 0; i < 2; i++) {
+            p.n[i] = n[i];
+            p.step[i] = steps[i];
+            if (p.step[i] < 0) p.from += p.step[i] * (p.n[i] - 1);
+            if (p.step[i] < 0) p.step[i] = -p.step[i];
+            if (p.step[i] == 0 || p.n[i] == 1) p.n[i] = p.step[i] = 1;
+        }
+        if (p.step[0] < p.step[1]) {
+            std::swap(p.step[0], p.step[1]);
+            std::swap(p.n[0], p.n[1]);
+        }
+        return p;
+    }
+    wide end() const { return from + step[0] * (n[0] - 1) + step[1] * (n[1] - 1) + size; }
+    bool operator==(const Pieces &o) const {
+        return from == o.from && size == o.size && n[0] == o.n[0] && n[1] == o.n[1] && (n[0] == 1 || step[0] == o.step[0]) && (n[1] == 1 || step[1] == o.step[1]);
+    }
+    // Whether one of these pieces starts within lo .. hi. Few i need a look where the pieces of one i end before the next i's.
+    bool starts_within(wide lo, wide hi) const {
+        lo -= from;
+        hi -= from;
+        const wide before = lo - step[1] * (n[1] - 1);
+        for (wide i = before > 0 ? (before + step[0] - 1) / step[0] : 0; i < n[0] && i * step[0] <= hi; i++) {
+            const wide at = lo - i * step[0];
+            const wide j = at > 0 ? (at + step[1] - 1) / step[1] : 0;
+            if (j < n[1] && i * step[0] + j * step[1] <= hi) return true;
+        }
+        return false;
+    }
+    // Whether any byte is in both; these pieces are apart from each other (check_written).
+    bool meets(const Pieces &o) const {
+        if (!n[0] || !o.n[0] || end() <= o.from || o.end() <= from) return false;
+        if (step[0] == o.step[0] && step[1] == o.step[1] && n[0] == o.n[0] && n[1] == o.n[1]) {
+            // rows of one kind: by the distances between two of them
+            Pieces d = *this;
+            for (int i = 0; i < 2; i++) {
+                d.from -= d.step[i] * (d.n[i] - 1);
+                d.n[i] = 2 * d.n[i] - 1;
+            }
+            return d.starts_within(o.from - size + 1, o.from + o.size - 1);
+        }
+        for (wide i = 0; i < o.n[0]; i++)
+            for (wide j = 0; j < o.n[1]; j++) {
+                const wide at = o.from + i * o.step[0] + j * o.step[1];
+                if (starts_within(at - size + 1, at + o.size - 1)) return true;
+            }
+        return false;
+    }
+};
+// A matrix: its whole outer steps, and the rows of one that is not whole.
+struct Memory {
+    Pieces part[2];
+    Memory() = default;
+    Memory(const void *data, wide bytes) : part{Pieces::array(data, bytes), Pieces()} {}
+    Memory(const zbpe_rows &m, int64_t rows, int64_t inner, int64_t cols) {
+        const int element = m.dtype == ZBPE_F32 || m.dtype == ZBPE_I32 ? 4 : m.dtype == ZBPE_I64 ? 8 : 2;
+        const wide bytes = (wide)cols * element, outer = (wide)m.outer_stride * element, step = (wide)m.inner_stride * element;
+        part[0] = Pieces::rows(m.data, bytes, rows / inner, outer, inner, step);
+        part[1] = Pieces::rows(m.data, bytes, 1, 1, rows % inner, step);
+        if (part[1].n[0]) part[1].from += outer * (rows / inner);
+    }
+    bool operator==(const Memory &o) const { return part[0] == o.part[0] && part[1] == o.part[1]; }
+    bool meets(const Memory &o) const {
+        return part[0].meets(o.part[0]) || part[0].meets(o.part[1]) || part[1].meets(o.part[0]) || part[1].meets(o.part[1]);
+    }
+};
+static zbpe_status apart(const char *what, const char *written, const Memory &w, const char *read, const Memory &r) {
+    return w.meets(r) ? refuse(ZBPE_INVALID_ARGUMENT, "%s: %s overlaps %s", what, written, read) : ZBPE_OK;
+}
+
+// The memory `w` that a call of adjust_logits or its gradient writes, against what it reads besides the logits.
+static zbpe_status apart_from_terms(const char *what, const char *written, const Memory &w, const zbpe_adjust &p) {
+    const wide rows = p.rows;
+    struct {
+        const char *name;
+        Memory r;
+    } const read[] = {
+        {"history", p.history_len ? Memory(p.history, p.rows, p.inner, p.history_len) : Memory()},
+        {"lengths", Memory(p.lengths, rows * 4)},
+        {"prompt_lengths", Memory(p.prompt_lengths, rows * 4)},
+        {"repetition", Memory(p.repetition, rows * 4)},
+        {"presence", Memory(p.presence, rows * 4)},
+        {"frequency", Memory(p.frequency, rows * 4)},
+        {"bias", Memory(p.bias, (wide)p.cols * 4)},
+        {"bias_tokens", Memory(p.bias_tokens, rows * p.n_biases * 4)},
+        {"bias_values", Memory(p.bias_values, rows * p.n_biases * 4)},
+        {"masks", Memory(p.masks, (wide)p.mask_rows * p.mask_words * 4)},
+        {"states", Memory(p.masks ? p.states : nullptr, rows * 4)},
+    };
+    for (const auto &x : read) {
+        const zbpe_status s = apart(what, written, w, x.name, x.r);
+        if (s != ZBPE_OK) return s;
+    }
+    return ZBPE_OK;
+}
+
 template <class F>
 static zbpe_status by_type(int dtype, F f) {
     return dtype == ZBPE_F32 ? f(float()) : dtype == ZBPE_F16 ? f(f16()) : f(bf16());
@@ -1578,6 +1693,12 @@ zbpe_status zbpe_grammar_masks(int device, void *stream, const zbpe_grammar *gra
     if (s != ZBPE_OK || !rows) return s;
     if (!masks) return refuse(ZBPE_INVALID_ARGUMENT, "%s: no masks", what);
     if (!g.index) return refuse(ZBPE_INVALID_ARGUMENT, "%s: no index of the tokens", what);
+    const Memory written(masks, (wide)rows * ((g.vocab + 31) / 32) * 4);
+    s = apart(what, "masks", written, "states", Memory(states, (wide)rows * 4));
+    if (s == ZBPE_OK) s = apart(what, "masks", written, "the automaton", Memory(g.next, (wide)g.n * 1024));
+    if (s == ZBPE_OK) s = apart(what, "masks", written, "the automaton", Memory(g.accepting, g.n));
+    if (s == ZBPE_OK) s = apart(what, "masks", written, "the index of the tokens", Memory(g.index, (wide)index_size(g.vocab)));
+    if (s != ZBPE_OK) return s;
     OnDevice on;
     if ((s = on.go(device)) != ZBPE_OK) return s;
     // a workgroup's slices share what it finds out about its state; few rows need many workgroups
@@ -1597,6 +1718,12 @@ zbpe_status zbpe_grammar_advance(int device, void *stream, const zbpe_grammar *g
     zbpe_status s = grammar_of(what, grammar, rows, &g);
     if (s != ZBPE_OK || !rows) return s;
     if (!states || !tokens || !out) return refuse(ZBPE_INVALID_ARGUMENT, "%s: an array is missing", what);
+    const Memory written(out, (wide)rows * 4);
+    if (out != states) s = apart(what, "out", written, "states", Memory(states, (wide)rows * 4));
+    if (s == ZBPE_OK && out != tokens) s = apart(what, "out", written, "tokens", Memory(tokens, (wide)rows * 4));
+    if (s == ZBPE_OK) s = apart(what, "out", written, "the automaton", Memory(g.next, (wide)g.n * 1024));
+    if (s == ZBPE_OK) s = apart(what, "out", written, "the automaton", Memory(g.accepting, g.n));
+    if (s != ZBPE_OK) return s;
     OnDevice on;
     if ((s = on.go(device)) != ZBPE_OK) return s;
     grammar_advance_kernel<<<grid_of((rows + 255) / 256), 256, 0, (hipStream_t)stream>>>(g, states, tokens, rows, out);
@@ -1609,6 +1736,12 @@ zbpe_status zbpe_adjust_logits(int device, void *stream, const zbpe_adjust *args
     zbpe_status s = adjust_of(what, args, &a);
     if (s == ZBPE_OK) s = check_written(what, "out", args->out, a.rows, a.inner, a.cols);
     if (s != ZBPE_OK || !a.rows) return s;
+    // in place each thread reads what it writes; otherwise a row that is loaded ahead could have been written already
+    const Memory written(args->out, a.rows, a.inner, a.cols);
+    const Memory logits(args->logits, a.rows, a.inner, a.cols);
+    if (!(written == logits)) s = apart(what, "out", written, "the logits", logits);
+    if (s == ZBPE_OK) s = apart_from_terms(what, "out", written, *args);
+    if (s != ZBPE_OK) return s;
     OnDevice on;
     if ((s = on.go(device)) != ZBPE_OK) return s;
     return by_type(args->logits.dtype, [&](auto ti) {
@@ -1639,6 +1772,11 @@ zbpe_status zbpe_adjust_logits_grad(int device, void *stream, const zbpe_adjust 
         if (grad_logits->dtype != args->logits.dtype) return refuse(ZBPE_INVALID_ARGUMENT, "%s: grad_logits has the type of the logits", what);
         s = check_written(what, "grad_logits", *grad_logits, g.a.rows, g.a.inner, g.a.cols);
         g.grad_logits = rows_of(*grad_logits);
+        const Memory written(*grad_logits, g.a.rows, g.a.inner, g.a.cols);
+        if (s == ZBPE_OK) s = apart(what, "grad_logits", written, "the logits", Memory(args->logits, g.a.rows, g.a.inner, g.a.cols));
+        if (s == ZBPE_OK)
+            s = apart(what, "grad_logits", written, "the output's gradient", Memory(args->out, g.a.rows, g.a.inner, g.a.cols));
+        if (s == ZBPE_OK) s = apart_from_terms(what, "grad_logits", written, *args);
     }
     if (s != ZBPE_OK) return s;
     if (grad_bias && workspace_size < zbpe_adjust_workspace(g.a.rows, g.a.cols))
@@ -1706,6 +1844,14 @@ zbpe_status zbpe_token_logprobs_grad(int device, void *stream, const zbpe_logpro
     if (!grad_logits || grad_logits->dtype != args->logits.dtype) return refuse(ZBPE_INVALID_ARGUMENT, "%s: grad_logits has the type of the logits", what);
     if ((s = check_written(what, "grad_logits", *grad_logits, a.rows, a.inner, a.cols)) != ZBPE_OK || !a.rows) return s;
     if (!grad || !a.stats) return refuse(ZBPE_INVALID_ARGUMENT, "%s: no gradient, or no stats", what);
+    const Memory written(*grad_logits, a.rows, a.inner, a.cols);
+    const Memory logits(args->logits, a.rows, a.inner, a.cols);
+    if (!(written == logits)) s = apart(what, "grad_logits", written, "the logits", logits);
+    if (s == ZBPE_OK) s = apart(what, "grad_logits", written, "the tokens", Memory(a.tokens, (wide)a.rows * (args->tokens_dtype == ZBPE_I64 ? 8 : 4)));
+    if (s == ZBPE_OK) s = apart(what, "grad_logits", written, "temperature", Memory(a.temperature, (wide)a.rows * 4));
+    if (s == ZBPE_OK) s = apart(what, "grad_logits", written, "grad", Memory(grad, (wide)a.rows * 4));
+    if (s == ZBPE_OK) s = apart(what, "grad_logits", written, "stats", Memory(a.stats, (wide)a.rows * 8));
+    if (s != ZBPE_OK) return s;
     a.grad = grad;
     a.grad_logits = rows_of(*grad_logits);
     OnDevice on;

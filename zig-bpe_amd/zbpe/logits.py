@@ -458,8 +458,8 @@ def adjust_logits(logits: torch.Tensor, *, history: Optional[torch.Tensor] = Non
     history: int32 or int64 [..., n]; lengths and prompt_lengths (int32 [...]): how many of a row's tokens count, and how
     many of these are the prompt's. History and bias tokens outside 0 .. V - 1 are passed over.
 
-    Gradients go to logits, bias and bias_values; tangents (forward mode) are refused. out: where to write (the logits' type or float32; it may be the logits
-    themselves), without gradients."""
+    Gradients go to logits, bias and bias_values; tangents (forward mode) are refused. out: where to write (the logits' type or
+    float32; it may be the logits themselves, and otherwise shares no memory with them or another argument), without gradients."""
     x = _Terms(history, lengths, prompt_lengths, repetition, presence, frequency, bias, bias_tokens, bias_values, masks, states)
     _is_tensor(logits, "logits")
     learns = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (logits, bias, bias_values))
