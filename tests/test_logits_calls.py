@@ -274,3 +274,28 @@ def test_out_beside_the_logits(kind):
         grammar.masks(states[:13], out=states.view(13, 10))
     torch.cuda.synchronize()
     assert torch.equal(buffer, was) and not bias.any() and not masks.any() and not states.any()
+
+
+# ---- numbers that stand for all rows -------------------------------------------------------------------------------------------
+
+
+@gpu
+def test_numbers_for_whole_values():
+    """a number for an int32 argument is whole and fits, or is refused; it is never cut off"""
+    z, x = adjust_case(4, 300, 1)
+    z, g, u = z.cuda(), to_gpu(x), torch.full((4,), 0.6, device="cuda")
+    for bad in (0.5, 1.5, -0.5, float("nan"), INF, -INF, 2 ** 31, 2 ** 40, -2 ** 31 - 1, 1e30):
+        with pytest.raises(zbpe.InvalidArgument, match="top_k"):
+            zbpe.draw_tokens(z, u, top_k=bad)
+        for name in ("lengths", "prompt_lengths"):
+            with pytest.raises(zbpe.InvalidArgument, match=name):
+                zbpe.adjust_logits(z, history=g["history"], **{name: bad})
+        with pytest.raises(zbpe.InvalidArgument, match="states"):
+            zbpe.adjust_logits(z, masks=g["masks"], states=bad)
+    whole = zbpe.draw_tokens(z, u, top_k=torch.full((4,), 3, dtype=torch.int32, device="cuda"))
+    for good in (3, 3.0):
+        assert torch.equal(zbpe.draw_tokens(z, u, top_k=good)[0], whole[0])
+    every = zbpe.draw_tokens(z, u)
+    for good in (0, -1, 2 ** 31 - 1, -2 ** 31, False):
+        assert torch.equal(zbpe.draw_tokens(z, u, top_k=good)[0], every[0])
+    zbpe.draw_tokens(z, u, temperature=1, top_p=1e300, min_p=0.5)  # (a float argument takes any number)

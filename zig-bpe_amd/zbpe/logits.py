@@ -8,7 +8,7 @@
 They run on libzbpe.so's kernels (include/zbpe.h states each one's definition), on the tensors' device and its current
 stream, wait for nothing and can be captured into a HIP graph. Logits are float32, float16 or bfloat16 with any number of
 leading axes, ``[..., V]`` with V up to 65536; a per-row tensor has the leading axes' shape, and a plain number stands for
-all rows. Tensors of the wrong type, shape or device raise InvalidArgument before anything is launched. Results of a captured
+all rows (a whole one for an int32 tensor). Tensors of the wrong type, shape or device raise InvalidArgument before anything is launched. Results of a captured
 call are those of the eager one, bit for bit; no result depends on the order in which workgroups run. A backward pass is captured
 as any of torch's: warmed up on a side stream, and while no eager graph of the same leaves is alive (torch ties a leaf's gradient
 to the stream that first used it).
@@ -150,6 +150,11 @@ class _Rows:
         if not isinstance(x, torch.Tensor):
             if not isinstance(x, (int, float)):
                 raise InvalidArgument(f"{name} is neither a tensor nor a number")
+            if dtype == torch.int32:
+                if not (-(2 ** 31) <= x < 2 ** 31 and x == int(x)):
+                    raise InvalidArgument(f"{name} is {x}, not a whole number of 32 bits")
+            elif abs(x) > 3.4e38:  # (rounded to 32 bits as a tensor's values are: infinite from half a step past the largest)
+                x = ctypes.c_float(min(max(x, -1e39), 1e39)).value
             x = torch.full(self.lead, x, dtype=dtype, device=self.device)
         elif x.dtype == dtype and x.shape == self.lead and x.get_device() == self.index and x.is_contiguous():
             return x.data_ptr()  # (the usual case; the caller holds it)
