@@ -386,7 +386,8 @@ zbpe_status zbpe_draw_tokens(int device, void *stream, const zbpe_draw *args);
 /* logprobs[r] = z[t] - log sum_v exp(z[v]) with z = logits[r] / temperature[r], t = tokens[r] (I32 or I64, packed). A negative
  * token is not scored: 0, and no gradient. A token past the last column gives NaN. A row without anything above -inf gives
  * -inf and no gradient. stats ([rows][2] f32: the row's maximum, and the sum of exp(z - its maximum)) is what the gradient
- * needs; it may be NULL when none follows. temperature: NULL: 1; positive.
+ * needs; it may be NULL when none follows. temperature: NULL: 1; what is below 2^-126 (0, negative, NaN, subnormal) counts as
+ * 2^-126; at an infinite one all logits above -inf weigh the same.
  * zbpe_token_logprobs_grad writes grad_logits (the logits' type; may be the logits themselves, as `out` above)
  * = grad[r] / temperature[r] * ([v == t] - softmax(z)[v]). */
 typedef struct zbpe_logprobs {

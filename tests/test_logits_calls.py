@@ -299,3 +299,75 @@ def test_numbers_for_whole_values():
     for good in (0, -1, 2 ** 31 - 1, -2 ** 31, False):
         assert torch.equal(zbpe.draw_tokens(z, u, top_k=good)[0], every[0])
     zbpe.draw_tokens(z, u, temperature=1, top_p=1e300, min_p=0.5)  # (a float argument takes any number)
+
+
+# ---- temperatures of log-probabilities -----------------------------------------------------------------------------------------
+
+
+@gpu
+@pytest.mark.parametrize("kind", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("cols", [300, 4099])
+def test_logprobs_at_any_temperature(cols, kind):
+    """From the smallest to infinite; 0, negative ones, NaN and subnormal ones count as 2^-126. Logits are eighths, so that no value
+    comes near the border of what 32 bits hold; one row spans more than 32 bits can (3e38 - -3e38).
+
+    An exponent e = d / T is off by 5 U |e|, and by what 1 / T loses where it is subnormal (half of 2^-149, twice in the scale,
+    relative to 1 / T); for T infinite it is |d| 2^-148 at most in place of 0."""
+    rng = np.random.default_rng(cols)
+    ts = np.float32([INF, 3e38, 1e38, 1e20, 1e3, 1e-3, 1e-20, 2e-38, 2.0 ** -126, 1e-38, 1e-40, 1e-45, 0.0, -1.0, float("nan")])
+    rows = 2 * len(ts)
+    z = torch.from_numpy(np.round(rng.standard_normal((rows, cols)) * 16) / 8).to(kind)
+    z[:, 5] = -INF
+    big = torch.finfo(kind).max * 0.9
+    z[:len(ts), 7], z[:len(ts), 9] = big, -big
+    z[:len(ts):2, 11] = big  # ties of the largest
+    tokens = torch.from_numpy(rng.choice([0, 5, 7, 9, 11, 20], rows))
+    tokens[len(ts):] = torch.from_numpy(rng.integers(0, cols, len(ts)))
+    tokens[len(ts) + 3] = -1
+    t32 = torch.from_numpy(np.tile(ts, 2))
+    up = torch.from_numpy(rng.uniform(-2, 2, rows)).float()
+    zg = z.cuda().requires_grad_()
+    y = zbpe.token_logprobs(zg, tokens.cuda(), temperature=t32.cuda())
+    got, = torch.autograd.grad(y, zg, up.cuda())
+
+    t = t32.double().numpy()[:, None]
+    t = np.where(t >= 2.0 ** -126, t, 2.0 ** -126)
+    d = z.double().numpy()
+    d = d - d.max(1, keepdims=True)
+    none = np.isneginf(d)
+    e = np.where(none, -np.inf, np.where(none, 0, d) / t)
+    w = np.exp(e)
+    p = w / w.sum(1, keepdims=True)
+    loss = np.where(np.isinf(t), 0.0, np.where(np.isinf(t), 0.0, t) * 2.0 ** -148)
+    off = np.where(p > 0, np.where(np.isinf(t), np.abs(np.where(none, 0, d)) * 2.0 ** -148, np.abs(np.where(p > 0, e, 0)) * (5 * U + loss)), 0.0)
+    mean = (p * off).sum(1)
+    at = np.arange(rows), np.maximum(tokens.numpy(), 0)
+    scored = tokens.numpy() >= 0
+    want = np.where(scored, np.where(none[at], -np.inf, e[at] - np.log(w.sum(1))), 0.0)
+    bound = np.where(scored & np.isfinite(want), U * (370 + 8 * np.abs(want)) + mean + np.abs(np.where(none[at], 0, d[at])) * 2.0 ** -148 + np.abs(
+        np.where(none[at], 0, e[at])) * loss[:, 0], 0)
+    with np.errstate(over="ignore"):
+        narrow = want.astype(np.float32).astype(np.float64)  # (past what 32 bits hold: -inf)
+    close(y, np.where(np.isinf(narrow), narrow, want), bound)
+    hot = np.zeros((rows, cols))
+    hot[at] = 1
+    g = np.where(scored, up.double().numpy() / t[:, 0], 0.0)[:, None]
+    want = g * (hot - p)
+    relative, least = half_step(kind)
+    rough = np.abs(g) * (p * (off + mean[:, None] + 370 * U) + (4 * U + loss) * (hot + p)) + np.abs(up.double().numpy())[:, None] * 2.0 ** -147
+    close(got, want, rough + (np.abs(want) + rough) * relative + least + np.abs(g) * 2.0 ** -126)
+    # one number for all rows
+    for number in (INF, 0.0, 0):
+        a = zbpe.token_logprobs(z.cuda(), tokens.cuda(), temperature=number)
+        b = zbpe.token_logprobs(z.cuda(), tokens.cuda(), temperature=torch.full((rows,), float(number), device="cuda"))
+        assert torch.equal(a.view(torch.int32), b.view(torch.int32)) and not a.isnan().any()
+
+
+@gpu
+def test_logprobs_of_a_draw_at_an_infinite_temperature():
+    """the log-probability that draw_tokens gives is the score of its token, masked tokens among the row"""
+    z = torch.randn(6, 700, device="cuda")
+    z[:, ::3] = -INF
+    tokens, logprobs = zbpe.draw_tokens(z, torch.rand(6, device="cuda"), temperature=INF)
+    # log of 466: 7 roundings of its sum of ones (exact), exponents within |d| 2^-148, one of logf (2 U relative), one more
+    np.testing.assert_allclose(zbpe.token_logprobs(z, tokens, temperature=INF).cpu().numpy(), logprobs.cpu().numpy(), rtol=8 * U, atol=0)

@@ -1269,6 +1269,13 @@ __device__ __forceinline__ int64_t token_of(const Logprobs &a, int64_t r) {
     return a.wide_ids ? ((const int64_t *)a.tokens)[r] : (int64_t)((const int32_t *)a.tokens)[r];
 }
 
+// 1 / temperature. What is below 2^-126, or not positive at all, counts as 2^-126; for an infinite one the least float stands
+// in place of 0, whose product with -inf would be NaN (any finite exponent is then below 2^-20).
+__device__ __forceinline__ float inverse_of(float temperature) { return fmaxf(1.0f / fmaxf(temperature, 0x1p-126f), 0x1p-149f); }
+// Half of z - top: the difference itself may be past what 32 bits hold (3e38 - -3e38) where temperatures are high. The same
+// bits as z - top otherwise.
+__device__ __forceinline__ float half_below(float z, float half_top) { return fmaf(z, 0.5f, -half_top); }
+
 // One pass with a running maximum and sum. TPR threads go over one row, AHEAD loads of 16 bytes each at a time. 8192 rows of 32000
 // bf16 in 122 us (0.52 GB, 4.3 TB/s; with one load at a time the kernel took 1.37 times as long). Short rows take a wave each. Bound
 // by memory.
@@ -1281,17 +1288,17 @@ __global__ __launch_bounds__(256) void logprobs_kernel(Logprobs a) {
         const int64_t r = r0 + threadIdx.x / TPR;
         const bool on = r < a.rows;
         const float temperature = on && a.temperature ? a.temperature[r] : 1.0f;
-        const float inverse = 1.0f / temperature, scale = inverse * LOG2E;
+        const float inverse = inverse_of(temperature), scale = 2 * (inverse * LOG2E);
         const T *row = on ? row_of<T>(a.logits, r, a.inner) : nullptr;
         float m = -INF, s = 0.0f;
         auto add = [&](const float *z, int n) {
             float more = m;
 #pragma unroll
             for (int e = 0; e < n; e++) more = fmaxf(more, z[e]);
-            const float from = more == -INF ? 0.0f : more;  // (nothing yet above -inf: the exponentials are 0, not NaN)
-            s *= __builtin_amdgcn_exp2f((m - from) * scale);
+            const float from = more == -INF ? 0.0f : 0.5f * more;  // (nothing yet above -inf: the exponentials are 0, not NaN)
+            s *= __builtin_amdgcn_exp2f(half_below(m, from) * scale);
 #pragma unroll
-            for (int e = 0; e < n; e++) s += __builtin_amdgcn_exp2f((z[e] - from) * scale);
+            for (int e = 0; e < n; e++) s += __builtin_amdgcn_exp2f(half_below(z[e], from) * scale);
             m = more;
         };
         if (on) {
@@ -1314,7 +1321,7 @@ __global__ __launch_bounds__(256) void logprobs_kernel(Logprobs a) {
             }
         }
         float top = wave_max(m);
-        s = wave_sum(s * __builtin_amdgcn_exp2f((m - (top == -INF ? 0.0f : top)) * scale));
+        s = wave_sum(s * __builtin_amdgcn_exp2f(half_below(m, top == -INF ? 0.0f : 0.5f * top) * scale));
         if (TPR > 64) {
             __syncthreads();
             if ((threadIdx.x & 63) == 0) {
@@ -1323,16 +1330,16 @@ __global__ __launch_bounds__(256) void logprobs_kernel(Logprobs a) {
             }
             __syncthreads();
             top = fmaxf(fmaxf(maxima[0], maxima[1]), fmaxf(maxima[2], maxima[3]));
-            const float from = top == -INF ? 0.0f : top;
+            const float from = top == -INF ? 0.0f : 0.5f * top;
             s = 0.0f;
 #pragma unroll
-            for (int w = 0; w < 4; w++) s += sums[w] * __builtin_amdgcn_exp2f((maxima[w] - from) * scale);
+            for (int w = 0; w < 4; w++) s += sums[w] * __builtin_amdgcn_exp2f(half_below(maxima[w], from) * scale);
         }
         if (on && t == 0) {
             const int64_t token = token_of(a, r);
             float y = 0.0f;
             if (token >= a.cols) y = __builtin_nanf("");
-            else if (token >= 0) y = s == 0.0f ? -INF : ((float)row[token] - top) * inverse - logf(s);
+            else if (token >= 0) y = s == 0.0f ? -INF : half_below((float)row[token], 0.5f * top) * (2 * inverse) - logf(s);
             a.logprobs[r] = y;
             if (a.stats) {
                 a.stats[2 * r] = top;
@@ -1357,8 +1364,8 @@ __global__ __launch_bounds__(256) void logprobs_grad_kernel(Logprobs a) {
         for (int c = 0; c < C; c++) x[c].load(row, first + c * 256 * N, a.cols);
         const int64_t token = token_of(a, r);
         const float temperature = a.temperature ? a.temperature[r] : 1.0f;
-        const float inverse = 1.0f / temperature, scale = inverse * LOG2E;
-        const float top = a.stats[2 * r], s = a.stats[2 * r + 1];
+        const float inverse = inverse_of(temperature), scale = 2 * (inverse * LOG2E);
+        const float half_top = 0.5f * a.stats[2 * r], s = a.stats[2 * r + 1];
         const bool scored = token >= 0 && s != 0.0f;
         const float g = scored ? a.grad[r] * inverse : 0.0f;
         const float less = token >= a.cols ? __builtin_nanf("") : g / s;
@@ -1369,7 +1376,7 @@ __global__ __launch_bounds__(256) void logprobs_grad_kernel(Logprobs a) {
             float z[N];
 #pragma unroll
             for (int e = 0; e < N; e++) {
-                const float d = scored ? -less * __builtin_amdgcn_exp2f((x[c].get(e) - top) * scale) : 0.0f;
+                const float d = scored ? -less * __builtin_amdgcn_exp2f(half_below(x[c].get(e), half_top) * scale) : 0.0f;
                 z[e] = col + e == token ? g + d : d;
             }
             store_floats<T, N>(out, col, a.cols, z);

@@ -554,7 +554,8 @@ class _Logprobs(torch.autograd.Function):
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, temperature=None) -> torch.Tensor:
     """float32 [...]: the log-probability of each row's token (int32 or int64 [...]) under softmax(logits / temperature), with
     the gradient with respect to the logits (tangents are refused). Negative tokens (padding) are not scored: 0, and no gradient. A token past the
-    last column gives NaN; so does +inf or NaN among the logits. A row of -inf alone gives -inf, and no gradient."""
+    last column gives NaN; so does +inf or NaN among the logits. A row of -inf alone gives -inf, and no gradient. A
+    temperature below 2^-126 (0, negative ones and NaN too) counts as 2^-126: all weight is the largest logits'."""
     _is_tensor(logits, "logits")
     if torch.is_grad_enabled():
         _no_gradient(temperature=temperature)
