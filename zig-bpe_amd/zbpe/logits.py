@@ -84,7 +84,7 @@ def _no_gradient(**named) -> None:
 def _no_tangent(**named) -> None:
     """No operator here has a forward-mode derivative. (A tensor with a tangent does not require a gradient, so that torch's own
     refusal is not reached; and no_grad does not switch tangents off.)"""
-    if forward_ad._current_level < 0 or not torch._C._is_fwd_grad_enabled():  # (the usual case: no tensor has one)
+    if not torch._C._is_fwd_grad_enabled():
         return
     for name, x in named.items():
         if isinstance(x, torch.Tensor) and forward_ad.unpack_dual(x).tangent is not None:
@@ -470,7 +470,9 @@ def adjust_logits(logits: torch.Tensor, *, history: Optional[torch.Tensor] = Non
     learns = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (logits, bias, bias_values))
     if torch.is_grad_enabled():
         _no_gradient(repetition=repetition, presence=presence, frequency=frequency)
-    _no_tangent(logits=logits, bias=bias, bias_values=bias_values, repetition=repetition, presence=presence, frequency=frequency, out=out)
+    if forward_ad._current_level >= 0:  # (otherwise no tensor has one)
+        _no_tangent(logits=logits, bias=bias, bias_values=bias_values, repetition=repetition, presence=presence, frequency=frequency,
+                    out=out)
     if out is not None:
         _is_tensor(out, "out")
         _need(not learns and not (out.requires_grad and torch.is_grad_enabled()), "out goes without gradients")
@@ -559,7 +561,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, temperature=No
     _is_tensor(logits, "logits")
     if torch.is_grad_enabled():
         _no_gradient(temperature=temperature)
-    _no_tangent(logits=logits, temperature=temperature)
+    if forward_ad._current_level >= 0:
+        _no_tangent(logits=logits, temperature=temperature)
     if torch.is_grad_enabled() and logits.requires_grad:
         return _Logprobs.apply(logits, tokens, temperature)
     return _logprobs(logits.detach(), tokens, temperature, None)
