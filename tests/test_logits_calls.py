@@ -371,3 +371,28 @@ def test_logprobs_of_a_draw_at_an_infinite_temperature():
     tokens, logprobs = zbpe.draw_tokens(z, torch.rand(6, device="cuda"), temperature=INF)
     # log of 466: 7 roundings of its sum of ones (exact), exponents within |d| 2^-148, one of logf (2 U relative), one more
     np.testing.assert_allclose(zbpe.token_logprobs(z, tokens, temperature=INF).cpu().numpy(), logprobs.cpu().numpy(), rtol=8 * U, atol=0)
+
+
+@gpu
+@pytest.mark.parametrize("temperature", [1.0, 0.7, 1.3])
+def test_logprobs_gradient_far_from_the_largest(temperature):
+    """32-bit logits that are eighths, so that their distances are exact, down to 80 temperatures below the largest: an element of
+    the gradient is off by its own few roundings there too. The exponential: 3 U (the instruction's 2, the correction's one);
+    the sum: 2 U, 3 U of the mean distance from the largest (below 3 here), and 4 + 6 additions and a rescaling; g / T, g / s,
+    their product and 1 / T: 5 U; together under 32 U."""
+    rng = np.random.default_rng(8)
+    cols = 256
+    z = torch.from_numpy(np.round(-rng.random((40, cols)) * 80 * temperature * 8) / 8).float()
+    z[:, 0] = 0
+    t = np.float64(np.float32(temperature))
+    e = z.double().numpy() / t
+    p = np.exp(e) / np.exp(e).sum(1, keepdims=True)
+    assert (-p * e).sum(1).max() < 3
+    tokens = torch.zeros(40, dtype=torch.int64)
+    zg = z.cuda().requires_grad_()
+    y = zbpe.token_logprobs(zg, tokens.cuda(), temperature=temperature)
+    got, = torch.autograd.grad(y, zg, torch.ones_like(y))
+    want = -p / t
+    got = got.double().cpu().numpy()
+    worst = (np.abs(got - want) / np.abs(want))[:, 1:].max() / U
+    assert worst < 32, worst
