@@ -3,7 +3,7 @@ tensors written in place, forward-mode derivatives, memory that overlaps, number
 
 Tolerances count roundings as test_logits.py does: u = 2^-24 for each 32-bit operation.
 """
-import ctypes
+import os
 import subprocess
 import sys
 
@@ -396,3 +396,19 @@ def test_logprobs_gradient_far_from_the_largest(temperature):
     got = got.double().cpu().numpy()
     worst = (np.abs(got - want) / np.abs(want))[:, 1:].max() / U
     assert worst < 32, worst
+
+
+# ---- without torch -------------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("blocked", [True, False])
+def test_the_tokenizer_does_not_need_torch(blocked):
+    """`from zbpe import *` takes the tokenizer alone, whether torch can be imported or not; the operators' names are there when
+    they are asked for"""
+    code = ("import sys\n" + ("sys.modules['torch'] = None\n" if blocked else "") + "from zbpe import *\nimport zbpe\n"
+            "assert BasicTokenizer is zbpe.BasicTokenizer and Merges().as_array() is not None\n"
+            "assert sys.modules.get('torch') is None\n"
+            + ("try:\n    zbpe.draw_tokens\nexcept ImportError:\n    print('fine')\n" if blocked else
+               "assert 'draw_tokens' in dir(zbpe) and zbpe.draw_tokens and sys.modules['torch']\nprint('fine')\n"))
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, env={**os.environ, "PYTHONPATH": os.path.dirname(os.path.dirname(zbpe.__file__))})
+    assert done.returncode == 0 and "fine" in done.stdout, done.stderr

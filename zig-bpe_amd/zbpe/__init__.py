@@ -705,11 +705,15 @@ _LOGITS = ("Vocabulary", "Grammar", "adjust_logits", "draw_tokens", "token_logpr
 
 
 def __getattr__(name: str):
-    if name in _LOGITS:  # (loaded when asked for: they need torch, the tokenizer does not)
+    if name in _LOGITS:  # (loaded when asked for, and left out of __all__: they need torch, the tokenizer does not)
         from . import logits
 
         return getattr(logits, name)
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+
+
+def __dir__():
+    return sorted({*globals(), *_LOGITS})
 
 
 __all__ = [
@@ -717,5 +721,4 @@ __all__ = [
     "OutOfMemory", "DeviceError", "InvalidToken", "InvalidFormat", "InvalidCharacter", "Overflow", "StreamTooLong",
     "InvalidArgument", "InternalError", "load_library", "synth_corpus", "comm_unique_id", "zig_order_winner",
     "merges_to_text", "format_time_stats", "vocabStart", "EXPORTS", "TRACE_COLUMNS", "torch_collective", "COLLECTIVE_FN",
-    "Vocabulary", "Grammar", "adjust_logits", "draw_tokens", "token_logprobs", "token_bytes",
 ]
