@@ -412,3 +412,23 @@ def test_the_tokenizer_does_not_need_torch(blocked):
                "assert 'draw_tokens' in dir(zbpe) and zbpe.draw_tokens and sys.modules['torch']\nprint('fine')\n"))
     done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, env={**os.environ, "PYTHONPATH": os.path.dirname(os.path.dirname(zbpe.__file__))})
     assert done.returncode == 0 and "fine" in done.stdout, done.stderr
+
+
+# ---- devices -------------------------------------------------------------------------------------------------------------------
+
+
+def test_a_grammar_needs_a_vocabulary_on_a_gpu():
+    v = zbpe.Vocabulary([(97, 98, 256)], 300, device="cpu")
+    assert v.lengths()[[0, 256, 299]].tolist() == [1, 2, 0]
+    with pytest.raises(zbpe.InvalidArgument, match="not on a GPU"):
+        zbpe.Grammar(v, torch.zeros(3, 256, dtype=torch.int32))
+
+
+@gpu
+def test_bits_per_byte_on_another_device():
+    v = zbpe.Vocabulary([(97, 98, 256)], 300, device="cpu")
+    z, tokens = torch.zeros(4, 300, device="cuda"), torch.tensor([1, 2, 256, -1], device="cuda")
+    with pytest.raises(zbpe.InvalidArgument, match="the vocabulary is on cpu"):
+        v.bits_per_byte(z, tokens)
+    there = zbpe.Vocabulary([(97, 98, 256)], 300, device="cuda")
+    np.testing.assert_allclose(float(there.bits_per_byte(z, tokens)), 3 * np.log2(300) / 4, rtol=400 * U)

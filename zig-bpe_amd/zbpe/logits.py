@@ -239,6 +239,9 @@ class Vocabulary:
         is not. logits [..., V] predict tokens [...]; negative tokens (padding) count for nothing. A 0-d float32 tensor, with a
         gradient with respect to the logits. A token past the vocabulary makes it NaN. (Its sums are torch's, which a captured
         graph does not replay safely: call it outside of one.)"""
+        _is_tensor(logits, "logits")
+        if logits.device != self.device:
+            raise InvalidArgument(f"logits are on {logits.device}, the vocabulary is on {self.device}")
         nats = token_logprobs(logits, tokens)
         known = (tokens >= 0) & (tokens < self.size)
         n = torch.where(known, self.lengths()[torch.where(known, tokens, 0).long()], 0).sum()
@@ -255,6 +258,8 @@ class Grammar:
     def __init__(self, vocabulary: Vocabulary, next, accepting=None):
         _need(isinstance(vocabulary, Vocabulary), "vocabulary is not a Vocabulary")
         device = vocabulary.device
+        if device.type != "cuda":
+            raise InvalidArgument(f"vocabulary is on {device}, not on a GPU")
         next = torch.as_tensor(next)
         if not (next.dim() == 2 and next.shape[1] == 256):
             raise InvalidArgument(f"next has shape {tuple(next.shape)} (states, 256)")
