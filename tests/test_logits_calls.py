@@ -432,3 +432,18 @@ def test_bits_per_byte_on_another_device():
         v.bits_per_byte(z, tokens)
     there = zbpe.Vocabulary([(97, 98, 256)], 300, device="cuda")
     np.testing.assert_allclose(float(there.bits_per_byte(z, tokens)), 3 * np.log2(300) / 4, rtol=400 * U)
+
+
+# ---- messages ------------------------------------------------------------------------------------------------------------------
+
+
+def test_an_older_message_is_not_taken_for_a_later_failure():
+    """zbpe_last_error(NULL) after a call without a context that has no message: not that of an operator's call before it"""
+    L = zbpe.load_library()
+    for fail in (lambda: L.zbpe_create(0, None), lambda: L.zbpe_comm_unique_id(None), lambda: L.zbpe_create_dist(0, 1, 1, None, None),
+                 lambda: L.zbpe_create_dist_host(0, 0, 0, zbpe.COLLECTIVE_FN(), None, None), lambda: L.zbpe_upload(None, None, 0),
+                 lambda: L.zbpe_tokens(None, None, 0, None), lambda: L.zbpe_zig_order_winner(None, None, None, 0, 0, 0, None)):
+        assert L.zbpe_adjust_logits(0, None, None) == 5 and b"no arguments" in L.zbpe_last_error(None)
+        assert fail() == 5
+        assert L.zbpe_last_error(None) == b"null context"
+    assert L.zbpe_draw_tokens(0, None, None) == 5 and b"zbpe_draw_tokens" in L.zbpe_last_error(None)

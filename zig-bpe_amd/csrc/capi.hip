@@ -14,6 +14,12 @@ struct zbpe_ctx {
     zbpe::Engine eng;
 };
 
+// A failure without a message of its own: where there is no context, an older call's message is not left to be taken for it.
+static zbpe_status refused(const zbpe_ctx *ctx = nullptr, zbpe_status s = ZBPE_INVALID_ARGUMENT) {
+    if (!ctx) zbpe::forget_thread_message();
+    return s;
+}
+
 static const char *env_or(const char *k) { const char *v = getenv(k); return v && *v ? v : nullptr; }
 
 extern "C" {
@@ -23,10 +29,10 @@ const char *zbpe_version(void) { return "zbpe-mi355x 0.3 (gfx950, zbpe_stats v3)
 size_t zbpe_stats_size(void) { return sizeof(zbpe_stats); }
 
 zbpe_status zbpe_create(int device, zbpe_ctx **out) {
-    if (!out) return ZBPE_INVALID_ARGUMENT;
+    if (!out) return refused();
     *out = nullptr;
     zbpe_ctx *c = new (std::nothrow) zbpe_ctx();
-    if (!c) return ZBPE_OUT_OF_MEMORY;
+    if (!c) return refused(nullptr, ZBPE_OUT_OF_MEMORY);
     zbpe_status s = c->eng.init(device);
     if (s != ZBPE_OK) {
         *out = c;  // keep it so zbpe_last_error() can report; caller destroys
@@ -42,9 +48,9 @@ zbpe_status zbpe_create(int device, zbpe_ctx **out) {
 }
 
 zbpe_status zbpe_comm_unique_id(void *out128) {
-    if (!out128) return ZBPE_INVALID_ARGUMENT;
+    if (!out128) return refused();
     ncclUniqueId id;
-    if (ncclGetUniqueId(&id) != ncclSuccess) return ZBPE_COMM_ERROR;
+    if (ncclGetUniqueId(&id) != ncclSuccess) return refused(nullptr, ZBPE_COMM_ERROR);
     memcpy(out128, &id, sizeof(id));
     return ZBPE_OK;
 }
@@ -56,7 +62,7 @@ static zbpe_status finish_dist(zbpe_ctx *c, int rank, int world, std::unique_ptr
 }
 
 zbpe_status zbpe_create_dist(int device, int rank, int world, const void *unique_id128, zbpe_ctx **out) {
-    if (!out || world < 1 || rank < 0 || rank >= world || (world > 1 && !unique_id128)) return ZBPE_INVALID_ARGUMENT;
+    if (!out || world < 1 || rank < 0 || rank >= world || (world > 1 && !unique_id128)) return refused();
     zbpe_status s = zbpe_create(device, out);
     if (s != ZBPE_OK || (world == 1 && !unique_id128)) return s;
     auto comm = std::make_unique<zbpe::RcclComm>();
@@ -66,7 +72,7 @@ zbpe_status zbpe_create_dist(int device, int rank, int world, const void *unique
 }
 
 zbpe_status zbpe_create_dist_host(int device, int rank, int world, zbpe_collective_fn fn, void *user, zbpe_ctx **out) {
-    if (!out || !fn || world < 1 || rank < 0 || rank >= world) return ZBPE_INVALID_ARGUMENT;
+    if (!out || !fn || world < 1 || rank < 0 || rank >= world) return refused();
     zbpe_status s = zbpe_create(device, out);
     if (s != ZBPE_OK) return s;
     auto comm = std::make_unique<zbpe::HostComm>();
@@ -87,19 +93,19 @@ const char *zbpe_last_error(const zbpe_ctx *ctx) {
 }
 
 zbpe_status zbpe_upload(zbpe_ctx *ctx, const uint8_t *text, size_t n) {
-    if (!ctx || (!text && n)) return ZBPE_INVALID_ARGUMENT;
+    if (!ctx || (!text && n)) return refused(ctx);
     return ctx->eng.upload(text, n, ctx->eng.multi());
 }
 
 zbpe_status zbpe_train_resident(zbpe_ctx *ctx, uint16_t vocab_size, int verbose, uint16_t *out_triples,
                                 uint64_t *out_counts, size_t *out_n_merges, zbpe_stats *stats) {
-    if (!ctx || !out_n_merges || (!out_triples && vocab_size > 256)) return ZBPE_INVALID_ARGUMENT;
+    if (!ctx || !out_n_merges || (!out_triples && vocab_size > 256)) return refused(ctx);
     return ctx->eng.train(vocab_size, verbose, out_triples, out_counts, out_n_merges, stats);
 }
 
 zbpe_status zbpe_train(zbpe_ctx *ctx, const uint8_t *text, size_t n, uint16_t vocab_size, int verbose,
                        uint16_t *out_triples, uint64_t *out_counts, size_t *out_n_merges, zbpe_stats *stats) {
-    if (!ctx || !out_n_merges || (!text && n)) return ZBPE_INVALID_ARGUMENT;
+    if (!ctx || !out_n_merges || (!text && n)) return refused(ctx);
     *out_n_merges = 0;
     if (vocab_size < 256) return ctx->eng.fail(ZBPE_INVALID_VOCAB_SIZE, "vocabSize %u < 256", vocab_size);
     zbpe_status s = ctx->eng.upload(text, n, ctx->eng.multi());
@@ -109,22 +115,22 @@ zbpe_status zbpe_train(zbpe_ctx *ctx, const uint8_t *text, size_t n, uint16_t vo
 
 zbpe_status zbpe_encode(zbpe_ctx *ctx, const uint16_t *triples, size_t n_merges, const uint8_t *text, size_t n,
                         uint16_t *out, size_t *out_len) {
-    if (!ctx || !out_len || (!text && n) || (!triples && n_merges) || (!out && n)) return ZBPE_INVALID_ARGUMENT;
+    if (!ctx || !out_len || (!text && n) || (!triples && n_merges) || (!out && n)) return refused(ctx);
     return ctx->eng.encode(triples, n_merges, text, n, out, out_len);
 }
 
 zbpe_status zbpe_verify_counts(zbpe_ctx *ctx, uint64_t *mismatches) {
-    if (!ctx || !mismatches) return ZBPE_INVALID_ARGUMENT;
+    if (!ctx || !mismatches) return refused(ctx);
     return ctx->eng.verify_counts(mismatches);
 }
 
 zbpe_status zbpe_tokens(zbpe_ctx *ctx, uint16_t *out, size_t cap, size_t *n_tokens) {
-    if (!ctx || !n_tokens || (!out && cap)) return ZBPE_INVALID_ARGUMENT;
+    if (!ctx || !n_tokens || (!out && cap)) return refused(ctx);
     return ctx->eng.tokens(out, cap, n_tokens);
 }
 
 zbpe_status zbpe_set_option(zbpe_ctx *ctx, const char *name, int64_t value) {
-    if (!ctx || !name) return ZBPE_INVALID_ARGUMENT;
+    if (!ctx || !name) return refused(ctx);
     std::string k(name);
     zbpe::Engine &e = ctx->eng;
     if (k == "debug_checks") e.debug_checks = value != 0;
@@ -190,7 +196,7 @@ zbpe_status zbpe_set_option(zbpe_ctx *ctx, const char *name, int64_t value) {
 // never materialises the pair array (the scan reads pairs in place), so generateCodePointPairs takes
 // 0 s over the count calls.
 zbpe_status zbpe_format_time_stats(const zbpe_stats *st, char *buf, size_t cap, size_t *len) {
-    if (!st || !len || (!buf && cap)) return ZBPE_INVALID_ARGUMENT;
+    if (!st || !len || (!buf && cap)) return refused();
     std::string out = "\nTime statistics:\n";
     auto line = [&](const char *name, double t, uint64_t calls) {
         char b[256], avg[64];
@@ -217,24 +223,24 @@ zbpe_status zbpe_format_time_stats(const zbpe_stats *st, char *buf, size_t cap, 
 }
 
 zbpe_status zbpe_bench_scan(zbpe_ctx *ctx, uint16_t a, uint16_t b, int reps, double *avg_ms, double *gbps) {
-    if (!ctx || !avg_ms || !gbps || reps < 1 || a == b) return ZBPE_INVALID_ARGUMENT;
+    if (!ctx || !avg_ms || !gbps || reps < 1 || a == b) return refused(ctx);
     return ctx->eng.bench_scan(a, b, reps, avg_ms, gbps);
 }
 
 zbpe_status zbpe_bench_train_scan(zbpe_ctx *ctx, int reps, int grid, double *avg_us, uint32_t *pair, uint32_t *list_len,
                                   int *mode) {
-    if (!ctx || !avg_us || !pair || !list_len || !mode || reps < 0 || grid < 0) return ZBPE_INVALID_ARGUMENT;
+    if (!ctx || !avg_us || !pair || !list_len || !mode || reps < 0 || grid < 0) return refused(ctx);
     return ctx->eng.bench_train_scan(reps, grid, avg_us, pair, list_len, mode);
 }
 
 zbpe_status zbpe_bench_recount(zbpe_ctx *ctx, int reps, double *avg_us, double *gbps, uint64_t *n_tokens,
                                uint64_t *mismatches) {
-    if (!ctx || !avg_us || !gbps || !n_tokens || !mismatches || reps < 0) return ZBPE_INVALID_ARGUMENT;
+    if (!ctx || !avg_us || !gbps || !n_tokens || !mismatches || reps < 0) return refused(ctx);
     return ctx->eng.bench_recount(reps, avg_us, gbps, n_tokens, mismatches);
 }
 
 zbpe_status zbpe_merge_log(zbpe_ctx *ctx, uint32_t *rows, size_t cap_rows, size_t *n_rows) {
-    if (!ctx || !n_rows || (!rows && cap_rows)) return ZBPE_INVALID_ARGUMENT;
+    if (!ctx || !n_rows || (!rows && cap_rows)) return refused(ctx);
     const auto &L = ctx->eng.h_log;
     *n_rows = std::min(ctx->eng.run.merges, L.size());
     const size_t k = std::min(cap_rows, *n_rows);
@@ -247,7 +253,7 @@ zbpe_status zbpe_merge_log(zbpe_ctx *ctx, uint32_t *rows, size_t cap_rows, size_
 }
 
 zbpe_status zbpe_trace(zbpe_ctx *ctx, float *rows, size_t cap_rows, size_t *n_rows) {
-    if (!ctx || !n_rows || (!rows && cap_rows)) return ZBPE_INVALID_ARGUMENT;
+    if (!ctx || !n_rows || (!rows && cap_rows)) return refused(ctx);
     const auto &t = ctx->eng.trace;
     *n_rows = t.size() / ZBPE_TRACE_COLS;
     const size_t k = std::min(cap_rows, *n_rows);
@@ -256,7 +262,7 @@ zbpe_status zbpe_trace(zbpe_ctx *ctx, float *rows, size_t cap_rows, size_t *n_ro
 }
 
 zbpe_status zbpe_scan_log(zbpe_ctx *ctx, int32_t *out, size_t cap, size_t *n) {
-    if (!ctx || !n || (!out && cap)) return ZBPE_INVALID_ARGUMENT;
+    if (!ctx || !n || (!out && cap)) return refused(ctx);
     const auto &l = ctx->eng.scan_log;
     *n = l.size();
     const size_t k = std::min(cap, *n);
@@ -265,7 +271,7 @@ zbpe_status zbpe_scan_log(zbpe_ctx *ctx, int32_t *out, size_t cap, size_t *n) {
 }
 
 zbpe_status zbpe_compaction_log(zbpe_ctx *ctx, uint32_t *rows, size_t cap_rows, size_t *n_rows) {
-    if (!ctx || !n_rows || (!rows && cap_rows)) return ZBPE_INVALID_ARGUMENT;
+    if (!ctx || !n_rows || (!rows && cap_rows)) return refused(ctx);
     const auto &l = ctx->eng.compact_log;
     *n_rows = l.size() / 2;
     const size_t k = std::min(cap_rows, *n_rows);
@@ -274,7 +280,7 @@ zbpe_status zbpe_compaction_log(zbpe_ctx *ctx, uint32_t *rows, size_t cap_rows, 
 }
 
 zbpe_status zbpe_halt_log(zbpe_ctx *ctx, uint32_t *rows, size_t cap_rows, size_t *n_rows) {
-    if (!ctx || !n_rows || (!rows && cap_rows)) return ZBPE_INVALID_ARGUMENT;
+    if (!ctx || !n_rows || (!rows && cap_rows)) return refused(ctx);
     const auto &l = ctx->eng.halt_log;
     *n_rows = l.size() / 3;
     const size_t k = std::min(cap_rows, *n_rows);
@@ -284,11 +290,11 @@ zbpe_status zbpe_halt_log(zbpe_ctx *ctx, uint32_t *rows, size_t cap_rows, size_t
 
 zbpe_status zbpe_zig_order_winner(const uint32_t *first_pos, const uint32_t *keys, const uint32_t *counts, size_t n,
                                   uint32_t top, int call_after_last_insert, uint32_t *winner) {
-    if ((!first_pos || !keys || !counts) && n) return ZBPE_INVALID_ARGUMENT;
-    if (!winner) return ZBPE_INVALID_ARGUMENT;
+    if ((!first_pos || !keys || !counts) && n) return refused();
+    if (!winner) return refused();
     std::vector<zbpe::ZigOrderInput> in(n);
     for (size_t i = 0; i < n; i++) in[i] = zbpe::ZigOrderInput{(uint64_t)first_pos[i], keys[i], counts[i]};
-    return zbpe::zig_order_winner(std::move(in), top, call_after_last_insert != 0, winner) ? ZBPE_OK : ZBPE_INTERNAL;
+    return zbpe::zig_order_winner(std::move(in), top, call_after_last_insert != 0, winner) ? ZBPE_OK : refused(nullptr, ZBPE_INTERNAL);
 }
 
 }  // extern "C"

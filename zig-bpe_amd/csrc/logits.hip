@@ -18,6 +18,7 @@ namespace zbpe {
 
 static thread_local char g_message[512] = "";
 const char *thread_message() { return g_message[0] ? g_message : nullptr; }
+void forget_thread_message() { g_message[0] = 0; }
 
 __attribute__((format(printf, 2, 3))) static zbpe_status refuse(zbpe_status s, const char *fmt, ...) {
     va_list ap;

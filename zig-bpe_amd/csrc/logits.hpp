@@ -2,5 +2,6 @@
 #pragma once
 
 namespace zbpe {
-const char *thread_message();  // of the calling thread's last failed call without a context; null: none yet
+const char *thread_message();  // of the calling thread's last failed call without a context; null: it has none
+void forget_thread_message();
 }
