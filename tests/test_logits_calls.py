@@ -447,3 +447,38 @@ def test_an_older_message_is_not_taken_for_a_later_failure():
         assert fail() == 5
         assert L.zbpe_last_error(None) == b"null context"
     assert L.zbpe_draw_tokens(0, None, None) == 5 and b"zbpe_draw_tokens" in L.zbpe_last_error(None)
+
+
+# ---- small uniform numbers -----------------------------------------------------------------------------------------------------
+
+
+@gpu
+def test_draw_by_a_very_small_uniform():
+    """The token is the first at which the sum exceeds u times the whole, exactly, also where u is no multiple of 2^-64: column 0
+    weighs x steps of 2^-47 beside 60000 columns of 2^47 steps, and u times the whole lies just above x, or just below it."""
+    cols = 60001
+    cases = []
+    for x in range(3, 4000):
+        z0 = np.float32(np.log(x * 2.0 ** -47))
+        near = np.exp(np.float64(z0)) * 2.0 ** 47
+        if abs(near - np.round(near)) > 0.25:  # (far from where the weight's own rounding turns)
+            continue
+        x = int(np.round(near))
+        whole = 60000 * 2 ** 47 + x
+        u = np.float32(x / whole)
+        if int(float(u).hex().split("p")[1]) > -41:
+            continue
+        for v in (u, np.nextafter(u, np.float32(1)), np.nextafter(u, np.float32(0))):
+            exact = int(float(v) * 2.0 ** 100) * whole  # (u is a multiple of 2^-100 here; times 2^100)
+            assert int(float(v) * 2.0 ** 100) == float(v) * 2.0 ** 100
+            first = 0 if x * 2 ** 100 > exact else 1
+            cut_off = 0 if x > (int(float(v) * 2.0 ** 64) * whole) >> 64 else 1
+            cases.append((z0, v, first, first != cut_off))
+    assert sum(c[3] for c in cases) > 20, "cases in which cutting u off at 2^-64 would draw another token"
+    cases = [c for c in cases if c[3]][:24] + cases[:24]
+    z = torch.zeros(len(cases), cols)
+    z[:, 0] = torch.tensor([float(c[0]) for c in cases])
+    tokens, _ = zbpe.draw_tokens(z.cuda(), torch.tensor([float(c[1]) for c in cases]).cuda())
+    assert tokens.tolist() == [c[2] for c in cases]
+    tiny = torch.tensor([2.0 ** -149, 2.0 ** -126, 2.0 ** -64, 0.0], device="cuda")
+    assert zbpe.draw_tokens(torch.zeros(4, 300, device="cuda"), tiny)[0].tolist() == [0] * 4

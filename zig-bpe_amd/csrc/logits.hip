@@ -1118,7 +1118,7 @@ struct Drawer {
 
     // Draws from the few pairs that can be left by the first k ranks (k > 0), or by the first that sum to `target`; false when
     // that would be more than NT, or not enough.
-    __device__ __forceinline__ bool few(float mine, int k, float p, double least_kept, uint64_t target, uint64_t scaled, uint64_t &whole) {
+    __device__ __forceinline__ bool few(float mine, int k, float p, double least_kept, uint64_t target, float u, uint64_t &whole) {
         // a threshold that `wanted` to 1.2 times as many threads' maxima reach
         const int wanted = k > 0 ? k : NT / 4;
         const uint32_t key = key_of(mine);
@@ -1150,7 +1150,7 @@ struct Drawer {
         const uint64_t by_id = sort(keep ? pair << 32 | pair >> 32 : 0, left);
         const float v = of_key((uint32_t)by_id);
         const uint64_t s = by_id ? mass(v) : 0;
-        const uint64_t from = scan(s, whole), t = __umul64hi(whole, scaled);
+        const uint64_t from = scan(s, whole), t = part_of_whole(u, whole);
         if (from <= t && t < from + s) sh.col = (int)~(uint32_t)(by_id >> 32);
         __syncthreads();
         return true;
@@ -1160,9 +1160,17 @@ struct Drawer {
         return t < 1 ? 1 : t > whole ? whole : t;
     }
 
+    // floor(u * whole) without rounding (below the whole): u = m * 2^-n with 24 bits of m, which stand at the product's top
+    __device__ __forceinline__ static uint64_t part_of_whole(float u, uint64_t whole) {
+        if (u >= 1.0f) return whole - 1;
+        if (!(u >= 0x1p-126f)) return 0;  // (the whole is below 2^64)
+        const uint32_t b = __float_as_uint(u), n = 126 - (b >> 23);  // u = 1/2 .. 1 times 2^-n
+        return __umul64hi(whole, (uint64_t)(b << 8 | 0x80000000u) << 32) >> min(n, 63u);
+    }
+
     __device__ __forceinline__ void draw(const Draw &a, int64_t r) {
         const float temperature = a.temperature ? a.temperature[r] : 1.0f, p = a.top_p ? a.top_p[r] : 1.0f;
-        const float least_f = a.min_p ? a.min_p[r] : 0.0f, u = a.uniforms[r];
+        const float least_f = a.min_p ? a.min_p[r] : 0.0f, u = uniform(a.uniforms[r]);
         const int k = a.top_k ? a.top_k[r] : 0;
         // the maximum of this thread's columns, and the first column that holds it
         float mine = -INF;
@@ -1203,8 +1211,6 @@ struct Drawer {
         scale = uniform(256 * 0x1.71547652b82fep0 / (double)temperature);
         cut = 0;
         const double least_kept = uniform(least_f > 0.0f ? least_f < 1.0f ? (double)least_f : 1.0 : 0.0);
-        // u * whole without rounding: u < 1 is a multiple of 2^-64 here (24 bits), and the product's high half its floor
-        const uint64_t scaled = u >= 1.0f ? ~0ull : u > 0.0f ? (uint64_t)((double)u * 18446744073709551616.0) : 0ull;
         const bool by_k = k > 0 && k < cols, by_p = p < 1.0f;
         bool untried = !by_k || k <= NT * 5 / 8;
         uint64_t whole;
@@ -1216,7 +1222,7 @@ struct Drawer {
             const bool sums = stage || !untried;
             if (sums) whole = uniform(part_sums());
             if (stage == 2) {
-                locate(__umul64hi(whole, scaled));
+                locate(part_of_whole(u, whole));
                 break;
             }
             const uint64_t target = stage ? target_of(p, whole) : (uint64_t)k;
@@ -1224,7 +1230,7 @@ struct Drawer {
                 untried = false;
                 uint64_t left;
                 floor = floor_of(temperature);
-                if (few(mine, by_k ? k : 0, p, least_kept, target, scaled, left)) {
+                if (few(mine, by_k ? k : 0, p, least_kept, target, u, left)) {
                     whole = left;
                     break;
                 }
