@@ -482,3 +482,18 @@ def test_draw_by_a_very_small_uniform():
     assert tokens.tolist() == [c[2] for c in cases]
     tiny = torch.tensor([2.0 ** -149, 2.0 ** -126, 2.0 ** -64, 0.0], device="cuda")
     assert zbpe.draw_tokens(torch.zeros(4, 300, device="cuda"), tiny)[0].tolist() == [0] * 4
+
+
+# ---- merge tables --------------------------------------------------------------------------------------------------------------
+
+
+def test_a_table_of_other_rows_is_no_table_of_triples():
+    """3 pairs are 6 numbers, as 2 triples are"""
+    for bad in ([[97, 98], [99, 100], [101, 102]], np.zeros((3, 2, 2), np.int64), np.zeros((3, 4), np.uint16), [[97] * 6]):
+        with pytest.raises(zbpe.InvalidArgument, match="triples"):
+            zbpe.token_bytes(bad)
+    want = zbpe.token_bytes([[97, 98, 256], [256, 99, 257]])
+    for good in ([97, 98, 256, 256, 99, 257], [[[97, 98, 256]], [[256, 99, 257]]]):
+        got = zbpe.token_bytes(good)
+        assert (got[0] == want[0]).all() and (got[1] == want[1]).all()
+    assert len(zbpe.token_bytes(np.zeros((0, 2)))[0]) == 257

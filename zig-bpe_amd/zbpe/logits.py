@@ -186,6 +186,7 @@ def _triples(merges) -> np.ndarray:
         merges = merges.as_array()
     a = np.asarray(merges)
     _need(a.size == 0 or (a.dtype.kind in "iu" and a.size % 3 == 0), "merges are triples of whole numbers: first, second, new token")
+    _need(a.ndim < 2 or a.shape[-1] == 3 or a.size == 0, "merges are triples of whole numbers: first, second, new token")
     _need(a.size == 0 or (a.min() >= 0 and a.max() <= 0xFFFF), "a merge's token is outside 0 .. 65535")
     return np.ascontiguousarray(a.reshape(-1, 3), dtype=np.uint16)
 
