@@ -13,7 +13,7 @@ import torch
 from torch.autograd import forward_ad
 
 import zbpe
-from test_logits import INF, U, adjust_case, close, cuda, gpu, half_step, kept_weights, pack, some_automaton, some_merges, to_gpu
+from test_logits import INF, U, adjust_case, check_draw, close, cuda, gpu, half_step, some_automaton, some_merges, to_gpu
 
 
 # ---- tensors that are written in place -----------------------------------------------------------------------------------------
@@ -497,3 +497,31 @@ def test_a_table_of_other_rows_is_no_table_of_triples():
         got = zbpe.token_bytes(good)
         assert (got[0] == want[0]).all() and (got[1] == want[1]).all()
     assert len(zbpe.token_bytes(np.zeros((0, 2)))[0]) == 257
+
+
+# ---- draws from many tokens ----------------------------------------------------------------------------------------------------
+
+
+@gpu
+@pytest.mark.parametrize("kind", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("cols", [700, 1024, 1025, 5000, 32000, 65536])
+@pytest.mark.parametrize("shape", ["normal", "levels", "flat", "steep"])
+def test_draw_with_large_cuts(shape, cols, kind):
+    """Cuts that leave more tokens than a workgroup has threads: by rank (top_k), by share (top_p), one after the other, and within
+    thousands of equal logits, where the cut lies between two ids. `steep`: all but a few logits lie in one narrow range."""
+    rng = np.random.default_rng(cols)
+    rows = 8
+    z = rng.standard_normal((rows, cols))
+    if shape == "levels":
+        z = np.round(z)
+    elif shape == "flat":
+        z = np.full((rows, cols), 0.25)
+    elif shape == "steep":
+        z = -2 + z * 1e-3
+        z[:, rng.integers(0, cols, 5)] = rng.integers(0, 3, (rows, 5))
+    z = torch.from_numpy(z).to(kind)
+    t = np.float32(1 + rng.random(rows))
+    k = np.int32([cols // 2, cols - 1, cols * 3 // 4, 641, 0, 0, cols * 7 // 8, 0])
+    p = np.float32([1.0, 1.0, 0.6, 1.0, 0.5, 0.9, 0.95, 0.97])
+    m = np.float32([0, 0, 0, 0, 0, 0, 0.01, 0.02])
+    check_draw(z, rng, t, k, p, m)
