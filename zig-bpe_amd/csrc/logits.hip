@@ -202,8 +202,9 @@ __device__ __forceinline__ int walk(const Automaton &g, int s, uint32_t at, uint
 // Each wave queues what is left and walks it 64 at a time. The rows of the automaton that such walks need most, the state's own
 // and up to three that follow it (seven: 3 % slower, since every state pays for them), are in shared memory, their entries
 // replaced by the places of these rows (0 .. ROWS - 1, then REFUSED, then all other states). The bits return to the order of ids in
-// shared memory. 2048 states x 65535 tokens in 168 us (a walk for each pair: 728), 600 x 32000 in 37; the 19 MB in and out would
-// take 4. What bounds it: the instructions of classifying and walking, then the latency of a state's rows.
+// shared memory. 2048 states x 65535 tokens in 172 us (a walk for each pair: 728), 600 x 32000 in 40; the 19 MB in and out would
+// take 4. What bounds it: the instructions of classifying and walking (vector instructions issue in 59 % of busy cycles) and, in
+// the rest, the latency of a state's rows, which every workgroup of a state prepares anew.
 template <int NT>
 __global__ __launch_bounds__(NT) void grammar_masks_kernel(Automaton g, const int32_t *states, int64_t rows, uint32_t *masks, int slices, int per) {
     constexpr int ROWS = 4, REFUSED = ROWS, SLICES = ZBPE_MAX_VOCAB / INDEX_SLICE, SLICE_WORDS = INDEX_SLICE / 32;
@@ -373,8 +374,10 @@ __global__ __launch_bounds__(256) void grammar_advance_kernel(Automaton g, const
 // A workgroup takes a slice of columns over a run of rows, 32 bytes of logits a thread. What a row needs from memory is on its
 // way while the row before it is worked on. The row's history is counted in shared memory: a bit for each column that is in it
 // (the bits of one load's columns in one byte, which is 0 for most loads) and how often behind the prompt. Whoever uses a bit
-// or a count clears it. Bound by memory: 4096 rows of 32000 bf16, up to 500 tokens of history each, in 146 us (0.52 GB, 3.6 TB/s; a
-// copy reaches 4.9), the gradient in 173.
+// or a count clears it. 4096 rows of 32000 bf16, up to 500 tokens of history each, in 149 us (0.52 GB, 3.5 TB/s; a copy
+// reaches 4.9), the gradient in 172. What bounds it: memory, with vector instructions in 55 % of busy cycles (the gradient: 41, and a
+// scattered load for each place of the history). 256 rows with histories up to 2000 take 30 us: a run is two rows, and each of
+// four slices counts all of a row's history, what lies behind the first 512 tokens within the row's turn.
 constexpr int ADJUST_THREADS = 512, ADJUST_PACKS = 2, ADJUST_RUN = 32;
 constexpr int ADJUST_GROUPS = 2;  // on a CU at a time: 4 waves on a SIMD leave 128 registers to a thread
 template <class T>
@@ -798,12 +801,13 @@ __device__ __forceinline__ float value_of(uint64_t pair) { return of_key((uint32
 __device__ __forceinline__ int col_of(uint64_t pair) { return (int)~(uint32_t)pair; }
 
 // One workgroup draws from one row, which it reads as often as the filters need (the first time from memory, then from the
-// caches: 1000 rows of 65535 floats in 122 us, 2.1 TB/s; kept in registers instead, a row leaves no room for a second
+// caches: 1000 rows of 65535 floats in 127 us, 2.1 TB/s; kept in registers instead, a row leaves no room for a second
 // workgroup on the CU, and 2.3 ms). The usual filters leave few tokens, and those are found without looking at every value
 // twice: with NT threads over interleaved columns, the k-th largest of the threads' maxima is no larger than the k-th largest
 // value, and little more than k values reach it. They go to one thread each, are sorted, cut, and drawn from. Only where more
 // than NT values would have to be looked at (a large k, a flat distribution) the cut is found by histograms over the row.
-// What bounds it: the exponentials of rows without top_k (about 25 operations of 64 bits for each value).
+// What bounds it: the exponentials of rows without top_k (vector instructions issue in 70 % of busy cycles; 44 a value, rows
+// with filters counted in). A single row is bound by the latency of one workgroup's steps: 32000 floats, all filters, in 23 us.
 template <class T, int NT>
 struct Drawer {
     static constexpr int N = Pack<T>::N, W = NT / 64, AHEAD = 4, BINS = 1024;
@@ -1303,7 +1307,7 @@ struct Exponent {
 };
 
 // One pass with a running maximum and sum. TPR threads go over one row, AHEAD loads of 16 bytes each at a time. 8192 rows of 32000
-// bf16 in 122 us (0.52 GB, 4.3 TB/s; with one load at a time the kernel took 1.37 times as long). Short rows take a wave each. Bound
+// bf16 in 121 us (0.52 GB, 4.3 TB/s; with one load at a time the kernel took 1.37 times as long). Short rows take a wave each. Bound
 // by memory.
 template <class T, int TPR>
 __global__ __launch_bounds__(256) void logprobs_kernel(Logprobs a) {
@@ -1376,7 +1380,7 @@ __global__ __launch_bounds__(256) void logprobs_kernel(Logprobs a) {
     }
 }
 
-// One slice of columns (blockIdx.y) of one row after another. 8192 rows of 32000 bf16 in 188 us (1.05 GB read and written, 5.6 TB/s
+// One slice of columns (blockIdx.y) of one row after another. 8192 rows of 32000 bf16 in 189 us (1.05 GB read and written, 5.5 TB/s
 // with what the caches keep of the forward pass; the loads come before the scalars that they do not need). Bound by memory.
 template <class T>
 __global__ __launch_bounds__(256) void logprobs_grad_kernel(Logprobs a) {
